@@ -120,6 +120,57 @@ RB_API int rb_fused_attn_hyb(const rb_attn_args* a, void* workspace, size_t ws_b
  *  - The array keeps the last call's contents; nothing in it needs to start at zero. */
 RB_API int rb_fused_attn_hyb_noalloc(const rb_attn_args* a, void* stream);
 
+/* ------------------------------------------------------------------ prompt attention
+ * Causal attention of whole prompts packed behind one another: sequence i is the
+ * tokens [cu[i], cu[i + 1]) (device int32 [B + 1], ascending) of q [T, H, D] and
+ * k, v [T, HK, D]; token t of a sequence attends to its tokens 0..t, head h to kv
+ * head h / (H / HK). out [T, H, D] of q's type. Rows of no sequence are written as
+ * zeros when zero_rest != 0 and left alone otherwise. fp32 accumulation and
+ * softmax statistics; a row's bits do not depend on the packing. Unit inner
+ * strides, other strides and bases in whole 16-byte pieces, D = 128,
+ * H / HK <= 64. No reference counterpart: its Prefill runs HF's SDPA
+ * (respect/alpamayo/model.py:73-132). */
+typedef struct rb_prompt_args {
+  int dtype;  /* RB_F32 or RB_BF16 */
+  int B, T, H, HK, D;
+  const void* q; int64_t sqt, sqh;
+  const void* k; int64_t skt, skh;
+  const void* v; int64_t svt, svh;
+  const int32_t* cu;
+  void* out; int64_t sot, soh;
+  float sm_scale;
+  int zero_rest;
+} rb_prompt_args;
+RB_API int rb_prompt_attn(const rb_prompt_args* a, void* stream);
+
+/* ------------------------------------------------------------------ paged attention
+ * Attention of one new token per batch entry over a paged cache: q, out
+ * [B, H, D]; k, v [pages, HK, page_size, D] (one layer of rb_kv_pages' store, or
+ * any strides); entry b reads the first lengths[r] + ahead tokens of table row
+ * r = seqs[b] (NULL: r = b), cut to [0, min(width * page_size, max_length)]
+ * (max_length 0: no further bound). A length of 0, a row outside [0, rows) and
+ * a sequence none of whose pages exist give zeros; entries outside [0, pages)
+ * name no page and their tokens are left out. The cache is cut into chunks at
+ * absolute positions whose size depends on the sequence's length alone, joined
+ * in order, so a row's bits do not depend on the batch. Unit inner strides, other
+ * strides and bases in whole 16-byte pieces, D = 128. */
+typedef struct rb_paged_args {
+  int dtype;  /* RB_F32 or RB_BF16 */
+  int B, H, HK, D;
+  const void* q; int64_t sqb, sqh;
+  const void* k; int64_t skp, skh, sks;
+  const void* v; int64_t svp, svh, svs;
+  int pages, page_size;
+  const int32_t* table; int64_t ld_table; int width, rows;
+  const int32_t* lengths;
+  const int32_t* seqs;
+  int ahead, max_length;
+  void* out; int64_t sob, soh;
+  float sm_scale;
+} rb_paged_args;
+RB_API size_t rb_paged_attn_workspace(const rb_paged_args* a);
+RB_API int rb_paged_attn(const rb_paged_args* a, void* workspace, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------ linear
  * out[M, N] = x[M, K] @ w[N, K]^T with a row-count-invariant reduction
  * (respect/kernels/gemm.py:11-41). x, w bf16 with unit inner stride; out
@@ -206,6 +257,80 @@ RB_API int rb_greedy_token(const void* logits, int dtype, int64_t ld, int M, int
 RB_API int rb_compact_kv(void* const* k_layers, void* const* v_layers, int n_layers, int HK, int D,
                   int64_t s_head, int64_t s_slot, int elem_bytes, const int32_t* src_slots, int n,
                   int dst_start, void* stream);
+
+/* ------------------------------------------------------------------ paged KV cache
+ * Pages of a KV cache shared by several sequences. `store` is one tensor
+ * [layers, 2 (K, V), pages, kv_heads, page_size, head_dim] (contiguous); sequence
+ * s holds the pages table[s, 0 .. held[s]) (row stride max_pages, -1 = none) and
+ * counts lengths[s] tokens, position t in slot t % page_size of its page
+ * t / page_size; refs[p] is the number of sequences that hold page p (0 = free).
+ * All of it is caller-owned device memory, so calls are asynchronous and
+ * capturable; calls on one cache must be ordered by the caller (one stream, or
+ * events). Lists hold at most RB_PAGES_MAX_LIST entries and name a sequence
+ * once. A call that cannot be served as a whole changes nothing and sets
+ * *status (first failure stands) to an rb_pages_status; of rb_kv_pages_write
+ * only the tokens concerned are left out. No reference counterpart: its buffer
+ * holds one sequence (kv_buffer.py:44-104).
+ *   reserve   room for counts[i] tokens after the committed ones: new pages are
+ *             the lowest free ones, in list order; a partly filled last page
+ *             that other sequences hold is copied first (the last of the list's
+ *             holders keeps it when nobody else does). Tokens written but not
+ *             committed before the call are not kept by such a copy.
+ *   write     tokens t in [offsets[i], offsets[i + 1]) (NULL: token i) go to
+ *             positions lengths[i] + t - offsets[i], inside reserved room.
+ *   commit    lengths[i] += counts[i], inside reserved room.
+ *   fork      an empty sequence dst[i] takes the tokens of src[i] (pages shared).
+ *   compact   kv_buffer.py:93-104 on pages: the written positions lengths[i] +
+ *             paths[i, j], j < counts[i] (strictly increasing) move to lengths[i]
+ *             + j in every layer and are committed; pages past them go back.
+ *   truncate  keep lengths[i] tokens (NULL: none, which frees the sequence),
+ *             the other pages go back, reserved ones too. */
+#define RB_PAGES_MAX_LIST 1024
+enum rb_pages_status {
+  RB_PAGES_OK = 0,
+  RB_PAGES_BAD_SEQUENCE = 1, /* a sequence that does not exist, is named twice, or a fork's target in use */
+  RB_PAGES_NONE_FREE = 2,    /* fewer free pages than the call needs */
+  RB_PAGES_BAD_COUNT = 3,    /* a count, length, path or position outside the sequence's room */
+  RB_PAGES_SHARED = 4        /* a write into a page that another sequence holds (reserve again after a fork) */
+};
+typedef struct rb_kv_pages {
+  void* store;
+  int layers, pages, kv_heads, page_size, head_dim, elem_bytes; /* head_dim * elem_bytes % 16 == 0, elem_bytes 2 or 4 */
+  int max_seqs, max_pages;
+  int32_t *table, *lengths, *held, *refs, *status;
+} rb_kv_pages;
+/* K and V [layers, tokens, kv_heads, head_dim] for layers layer0 .. of the
+ * cache; strides in elements, unit inner stride, in whole 16-byte pieces. */
+typedef struct rb_kv_tokens {
+  const void *k, *v;
+  int64_t skl, skt, skh, svl, svt, svh;
+  int layer0, layers, tokens;
+} rb_kv_tokens;
+RB_API size_t rb_kv_pages_workspace(const rb_kv_pages* c);
+RB_API int rb_kv_pages_reserve(const rb_kv_pages* c, const int32_t* seqs, const int32_t* counts, int n, void* workspace,
+                               size_t ws_bytes, void* stream);
+RB_API int rb_kv_pages_write(const rb_kv_pages* c, const rb_kv_tokens* x, const int32_t* seqs, const int32_t* offsets,
+                             int n, void* stream);
+RB_API int rb_kv_pages_commit(const rb_kv_pages* c, const int32_t* seqs, const int32_t* counts, int n, void* stream);
+RB_API int rb_kv_pages_fork(const rb_kv_pages* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
+                            size_t ws_bytes, void* stream);
+RB_API int rb_kv_pages_compact(const rb_kv_pages* c, const int32_t* seqs, const int32_t* paths, int64_t ld_paths,
+                               int width, const int32_t* counts, int n, void* workspace, size_t ws_bytes, void* stream);
+RB_API int rb_kv_pages_truncate(const rb_kv_pages* c, const int32_t* seqs, const int32_t* lengths, int n, void* stream);
+
+/* ------------------------------------------------------------------ token log probabilities
+ * Per row m of logits [M, V] (RB_F32 or RB_BF16, row stride ld) with
+ * [offset, offset + size) excluded (as rb_greedy_token): logprob[m] =
+ * log softmax(row)[tokens[m]], entropy[m] = -sum p log p, and, for top > 0, the
+ * top entries by value, ties to the lowest index (NaN first, excluded entries
+ * count as -inf): top_ids [M, top], top_logprobs [M, top]. A row with a NaN, a
+ * +inf or no finite entry gives NaN log probabilities and entropy; a token
+ * outside [0, V) gives NaN, an excluded one -inf. top <= 32 and <= V. */
+#define RB_LOGPROBS_MAX_TOP 32
+RB_API size_t rb_token_logprobs_workspace(int M, int V, int top);
+RB_API int rb_token_logprobs(const void* logits, int dtype, int64_t ld, int M, int V, const int64_t* tokens, int offset,
+                             int size, int top, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,
+                             void* workspace, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------ trie masks
  * parents: device int32 [q], parents[i] < i or -1 for a root (trie.py:31-48

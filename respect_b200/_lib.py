@@ -21,6 +21,8 @@ RB_F32, RB_BF16, RB_U8, RB_I32, RB_I64 = 0, 1, 2, 3, 4
 RB_MASK_BOOL, RB_MASK_ADD_BF16, RB_MASK_ADD_F32, RB_MASK_CAUSAL = 0, 1, 2, 3
 COMPACT_MAX_LAYERS = 128
 COMPACT_MAX_SLOTS = 1024
+LOGPROBS_MAX_TOP = 32
+PAGES_MAX_LIST = 1024
 
 _DT = {torch.float32: RB_F32, torch.bfloat16: RB_BF16, torch.uint8: RB_U8, torch.bool: RB_U8,
        torch.int32: RB_I32, torch.int64: RB_I64}
@@ -52,6 +54,43 @@ class AttnArgs(ctypes.Structure):
                 ("sm_scale", c_float)]
 
 
+class PromptArgs(ctypes.Structure):
+    """Mirror of rb_prompt_args."""
+    _fields_ = [("dtype", c_int), ("B", c_int), ("T", c_int), ("H", c_int), ("HK", c_int), ("D", c_int),
+                ("q", c_void_p), ("sqt", c_int64), ("sqh", c_int64),
+                ("k", c_void_p), ("skt", c_int64), ("skh", c_int64),
+                ("v", c_void_p), ("svt", c_int64), ("svh", c_int64),
+                ("cu", c_void_p), ("out", c_void_p), ("sot", c_int64), ("soh", c_int64),
+                ("sm_scale", c_float), ("zero_rest", c_int)]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of rb_paged_args."""
+    _fields_ = [("dtype", c_int), ("B", c_int), ("H", c_int), ("HK", c_int), ("D", c_int),
+                ("q", c_void_p), ("sqb", c_int64), ("sqh", c_int64),
+                ("k", c_void_p), ("skp", c_int64), ("skh", c_int64), ("sks", c_int64),
+                ("v", c_void_p), ("svp", c_int64), ("svh", c_int64), ("svs", c_int64),
+                ("pages", c_int), ("page_size", c_int),
+                ("table", c_void_p), ("ld_table", c_int64), ("width", c_int), ("rows", c_int),
+                ("lengths", c_void_p), ("seqs", c_void_p), ("ahead", c_int), ("max_length", c_int),
+                ("out", c_void_p), ("sob", c_int64), ("soh", c_int64), ("sm_scale", c_float)]
+
+
+class KVPages(ctypes.Structure):
+    """Mirror of rb_kv_pages."""
+    _fields_ = [("store", c_void_p), ("layers", c_int), ("pages", c_int), ("kv_heads", c_int), ("page_size", c_int),
+                ("head_dim", c_int), ("elem_bytes", c_int), ("max_seqs", c_int), ("max_pages", c_int),
+                ("table", c_void_p), ("lengths", c_void_p), ("held", c_void_p), ("refs", c_void_p),
+                ("status", c_void_p)]
+
+
+class KVTokens(ctypes.Structure):
+    """Mirror of rb_kv_tokens."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("skl", c_int64), ("skt", c_int64), ("skh", c_int64),
+                ("svl", c_int64), ("svt", c_int64), ("svh", c_int64), ("layer0", c_int), ("layers", c_int),
+                ("tokens", c_int)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "rb_status_string": (ctypes.c_char_p, [c_int]),
@@ -81,6 +120,21 @@ SIGNATURES = {
     "rb_compact_kv": (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), c_int, c_int, c_int,
                               c_int64, c_int64, c_int, ctypes.POINTER(ctypes.c_int32), c_int, c_int,
                               c_void_p]),
+    "rb_prompt_attn": (c_int, [ctypes.POINTER(PromptArgs), c_void_p]),
+    "rb_paged_attn_workspace": (c_size_t, [ctypes.POINTER(PagedArgs)]),
+    "rb_paged_attn": (c_int, [ctypes.POINTER(PagedArgs), c_void_p, c_size_t, c_void_p]),
+    "rb_kv_pages_workspace": (c_size_t, [ctypes.POINTER(KVPages)]),
+    "rb_kv_pages_reserve": (c_int, [ctypes.POINTER(KVPages), c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "rb_kv_pages_write": (c_int, [ctypes.POINTER(KVPages), ctypes.POINTER(KVTokens), c_void_p, c_void_p, c_int,
+                                  c_void_p]),
+    "rb_kv_pages_commit": (c_int, [ctypes.POINTER(KVPages), c_void_p, c_void_p, c_int, c_void_p]),
+    "rb_kv_pages_fork": (c_int, [ctypes.POINTER(KVPages), c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "rb_kv_pages_compact": (c_int, [ctypes.POINTER(KVPages), c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int,
+                                    c_void_p, c_size_t, c_void_p]),
+    "rb_kv_pages_truncate": (c_int, [ctypes.POINTER(KVPages), c_void_p, c_void_p, c_int, c_void_p]),
+    "rb_token_logprobs_workspace": (c_size_t, [c_int, c_int, c_int]),
+    "rb_token_logprobs": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "rb_trie_node_mask": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
     "rb_verify_mask": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
 }
@@ -128,6 +182,24 @@ def stream_of(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise ValueError("respect_b200 operators take CUDA tensors (no CPU path)")
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call an entry point with the current stream of t's device as its last argument, that device being current."""
+    st = stream_of(t)
+    if t.device.index == torch.cuda.current_device():
+        call(name, *args, st)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args, st)
+
+
+def scratch(t: torch.Tensor, nbytes: int) -> torch.Tensor | None:
+    """Scratch for one call on the current stream (torch's allocator owns it: calls captured into
+    different graphs never share it)."""
+    if nbytes <= 0:
+        return None
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device)
 
 
 _ws: dict = {}

@@ -52,6 +52,14 @@ int rb_fused_attn_hyb(const rb_attn_args* a, void* workspace, size_t ws_bytes, v
   return attn_launch(a, workspace, ws_bytes, as_stream(stream));
 }
 
+int rb_prompt_attn(const rb_prompt_args* a, void* stream) { return prompt_launch(a, as_stream(stream)); }
+
+size_t rb_paged_attn_workspace(const rb_paged_args* a) { return paged_workspace(a); }
+
+int rb_paged_attn(const rb_paged_args* a, void* workspace, size_t ws_bytes, void* stream) {
+  return paged_launch(a, workspace, ws_bytes, as_stream(stream));
+}
+
 // ------------------------------------------------------------------ linear
 size_t rb_linear_workspace(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
@@ -196,6 +204,53 @@ int rb_compact_kv(void* const* k_layers, void* const* v_layers, int n_layers, in
   if (elem_bytes != 2 && elem_bytes != 4) return RB_ERR_UNSUPPORTED;
   return compact_launch(k_layers, v_layers, n_layers, HK, D, s_head, s_slot, elem_bytes, src_slots, n, dst_start,
                         as_stream(stream));
+}
+
+// ------------------------------------------------------------------ paged KV cache
+size_t rb_kv_pages_workspace(const rb_kv_pages* c) { return kv_pages_workspace(c); }
+
+int rb_kv_pages_reserve(const rb_kv_pages* c, const int32_t* seqs, const int32_t* counts, int n, void* workspace,
+                        size_t ws_bytes, void* stream) {
+  return kv_pages_reserve(c, seqs, counts, n, workspace, ws_bytes, as_stream(stream));
+}
+
+int rb_kv_pages_write(const rb_kv_pages* c, const rb_kv_tokens* x, const int32_t* seqs, const int32_t* offsets, int n,
+                      void* stream) {
+  return kv_pages_write(c, x, seqs, offsets, n, as_stream(stream));
+}
+
+int rb_kv_pages_commit(const rb_kv_pages* c, const int32_t* seqs, const int32_t* counts, int n, void* stream) {
+  return kv_pages_commit(c, seqs, counts, n, as_stream(stream));
+}
+
+int rb_kv_pages_fork(const rb_kv_pages* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
+                     size_t ws_bytes, void* stream) {
+  return kv_pages_fork(c, src, dst, n, workspace, ws_bytes, as_stream(stream));
+}
+
+int rb_kv_pages_compact(const rb_kv_pages* c, const int32_t* seqs, const int32_t* paths, int64_t ld_paths, int width,
+                        const int32_t* counts, int n, void* workspace, size_t ws_bytes, void* stream) {
+  return kv_pages_compact(c, seqs, paths, ld_paths, width, counts, n, workspace, ws_bytes, as_stream(stream));
+}
+
+int rb_kv_pages_truncate(const rb_kv_pages* c, const int32_t* seqs, const int32_t* lengths, int n, void* stream) {
+  return kv_pages_truncate(c, seqs, lengths, n, as_stream(stream));
+}
+
+// ------------------------------------------------------------------ token log probabilities
+size_t rb_token_logprobs_workspace(int M, int V, int top) { return logprobs_workspace(M, V, top); }
+
+int rb_token_logprobs(const void* logits, int dtype, int64_t ld, int M, int V, const int64_t* tokens, int offset,
+                      int size, int top, float* logprob, float* entropy, float* top_logprobs, int64_t* top_ids,
+                      void* workspace, size_t ws_bytes, void* stream) {
+  if (M < 0 || V <= 0 || ld < V || size < 0 || offset < 0 || top < 0 || top > V) return RB_ERR_INVALID_ARG;
+  if (top > RB_LOGPROBS_MAX_TOP) return RB_ERR_CAPACITY;
+  if (dtype != RB_F32 && dtype != RB_BF16) return RB_ERR_UNSUPPORTED;
+  if (M == 0) return RB_OK;
+  if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprobs || !top_ids))) return RB_ERR_INVALID_ARG;
+  if (!workspace || ws_bytes < logprobs_workspace(M, V, top) || !aligned16(workspace)) return RB_ERR_WORKSPACE;
+  return logprobs_launch(logits, dtype, ld, M, V, tokens, offset, size, top, logprob, entropy, top_logprobs, top_ids,
+                         workspace, as_stream(stream));
 }
 
 int rb_trie_node_mask(const int32_t* parents, int q, int committed, int M, int NN, uint8_t* msk, int64_t ld,

@@ -6,6 +6,10 @@
 #include "attention_tc.cu"
 #include "attention.cu"
 #include "attention_noalloc.cu"
+#include "attention_paged.cu"
+#include "attention_prompt.cu"
 #include "elementwise.cu"
+#include "kv_pages.cu"
+#include "logprobs.cu"
 #include "capi.cu"
 #include "engine.cu"

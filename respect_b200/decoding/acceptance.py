@@ -1,13 +1,14 @@
-"""Greedy token choice and the acceptance walk over a verified trie.
+"""Greedy token choice, token log probabilities and the acceptance walk over a verified trie.
 
 Mirror of ``respect.decoding.acceptance`` (respect/decoding/acceptance.py:11-46).
 `greedy_token` runs on the device (rb_greedy_token): the action-vocabulary range
 is skipped inside the argmax instead of materialising a masked fp32 clone of
-the [q, vocab] logits.
+the [q, vocab] logits. `token_logprobs` (rb_token_logprobs) says how likely given
+tokens were under the same exclusion, with the entropy and the best alternatives.
 """
 from __future__ import annotations
 
-from typing import Callable
+from typing import Callable, NamedTuple
 
 import torch
 
@@ -31,6 +32,47 @@ def greedy_token(logits: torch.Tensor, offset: int, size: int) -> torch.Tensor:
     _lib.call("rb_greedy_token", x2.data_ptr(), _lib.dtype_code(x2.dtype), x2.stride(0), M, V,
               int(offset), int(size), out.data_ptr(), _lib.stream_of(x2))
     return out.reshape(x.shape[:-1])
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor                 # fp32 [rows]: log softmax at the given token
+    entropy: torch.Tensor                 # fp32 [rows], in nats
+    top_logprobs: torch.Tensor | None     # fp32 [rows, top], descending
+    top_ids: torch.Tensor | None          # int64 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, offset: int = 0,
+                   size: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens`` (int64, one per row of ``logits`` [..., vocab], fp32 or bf16),
+    the rows' entropy and their ``top`` (at most 32) best entries, ties to the lowest index, with
+    [offset, offset + size) excluded as in greedy_token (-inf for an excluded token; excluded
+    entries follow the others among the alternatives). A row holding NaN or +inf, or nothing but
+    -inf, gives NaN, and so does a token outside the vocabulary."""
+    if logits.dim() == 0 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("token_logprobs takes fp32 or bf16 logits [..., vocab]")
+    V = logits.shape[-1]
+    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1] or tokens.device != logits.device:
+        raise ValueError(f"tokens must be int64 {tuple(logits.shape[:-1])} on {logits.device}")
+    if not 0 <= top <= min(_lib.LOGPROBS_MAX_TOP, V):
+        raise ValueError(f"top must be between 0 and {min(_lib.LOGPROBS_MAX_TOP, V)}")
+    if offset < 0 or size < 0 or V == 0:
+        raise ValueError("token_logprobs: bad excluded range or empty vocabulary")
+    x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
+    x = x.reshape(-1, V)
+    M, dev = x.shape[0], x.device
+    tok = tokens.reshape(-1).contiguous()
+    lp, ent = torch.empty(2, M, dtype=torch.float32, device=dev).unbind(0)
+    tlp = torch.empty(M, top, dtype=torch.float32, device=dev) if top else None
+    ids = torch.empty(M, top, dtype=torch.int64, device=dev) if top else None
+    nbytes = _lib.lib().rb_token_logprobs_workspace(M, V, top)
+    ws = _lib.scratch(x, nbytes)
+    _lib.launch("rb_token_logprobs", x, x.data_ptr(), _lib.dtype_code(x.dtype), x.stride(0) if M > 1 else V, M, V,
+                tok.data_ptr(), min(int(offset), V), min(int(size), V), int(top), lp.data_ptr(), ent.data_ptr(),
+                tlp.data_ptr() if top else None, ids.data_ptr() if top else None,
+                ws.data_ptr() if ws is not None else None, nbytes)
+    lead = tokens.shape
+    return TokenLogprobs(lp.reshape(lead), ent.reshape(lead), tlp.reshape(*lead, top) if top else None,
+                         ids.reshape(*lead, top) if top else None)
 
 
 def walk(tree: Trie, first: int, cap: int, eos: int,

@@ -1,12 +1,19 @@
-"""Trie-verification attention with a slot-order-independent node sum.
+"""Trie-verification attention with a slot-order-independent node sum, and the attention of
+whole prompts and of single new tokens beside it.
 
-Drop-in for ``respect.kernels.attention.fused_attn_hyb``
+`fused_attn_hyb` is a drop-in for ``respect.kernels.attention.fused_attn_hyb``
 (respect/kernels/attention.py:74-96): same argument names, shapes and output.
 The tile keyword arguments (BM, BN, num_warps, num_stages) of the Triton
 version are accepted and ignored; BNB keeps the reference's divisibility
 check on the node count. The computation runs in librespect_b200.so
 (rb_fused_attn_hyb): prefix keys in fixed chunks at absolute positions,
 nodes one at a time in slot order, fp32 accumulation, one final cast.
+
+`prompt_attention` (rb_prompt_attn) is causal attention over packed whole prompts;
+`paged_attention` (rb_paged_attn) reads one new token's keys from a paged cache
+(respect_b200.decoding.kv_pages). Both take bf16 or fp32, any number of query heads
+per kv head that divides evenly, head size 128, and keep the property of the trie
+kernel: what a sequence gets does not depend on what else the call carries.
 """
 from __future__ import annotations
 
@@ -68,3 +75,112 @@ def fused_attn_hyb(q, kp, vp, kn, vn, msk, sm_scale=None,
     q, kp, vp, kn, vn = (_unit_inner(t) for t in (q, kp, vp, kn, vn))
     out = torch.empty_like(q)
     return attn_call(q, kp, vp, kn, vn, msk, out, sm_scale)
+
+
+def _rows(t: torch.Tensor, name: str, dims: int, like: torch.Tensor) -> torch.Tensor:
+    """t with the layout the kernels read (unit inner stride, rows in whole 16-byte pieces); a copy only if it lacks it."""
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    unit = 16 // t.element_size()
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % unit or s < 0 for s in st[:-1]):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _out(out, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    unit = 16 // q.element_size()
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
+    if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % unit for s in out.stride()[:-1]):
+        raise ValueError("out needs a unit inner stride and rows in whole 16-byte pieces")
+    return out
+
+
+def _int32(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != dims:
+        raise TypeError(f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    return t
+
+
+def _check_heads(q: torch.Tensor, heads_kv: int, dim: int) -> None:
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"attention takes bf16 or fp32, got {q.dtype}")
+    if dim != 128 or q.shape[-1] != 128:
+        raise ValueError("attention heads must have 128 dims")
+    if heads_kv == 0 or q.shape[1] == 0 or q.shape[1] % heads_kv:
+        raise ValueError(f"{q.shape[1]} query heads do not share {heads_kv} kv heads evenly")
+
+
+def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
+    """Causal attention over whole prompts packed behind one another.
+
+    q [T, H, 128], k, v [T, HK, 128] (bf16 or fp32; slices of a fused projection are
+    read in place), cu_seqlens int32 [B + 1] on the same device: sequence i is tokens
+    [cu_seqlens[i], cu_seqlens[i + 1]), ascending. Returns [T, H, 128]. Rows of no
+    sequence are zero in a new result and left as they were in a given ``out``."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0]:
+        raise ValueError(f"prompt_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
+    _check_heads(q, k.shape[1], k.shape[2])
+    if q.shape[1] // k.shape[1] > 64:
+        raise ValueError("prompt_attention: at most 64 query heads per kv head")
+    cu = _int32(cu_seqlens, "cu_seqlens", 1, q.device)
+    if cu.numel() < 1:
+        raise ValueError("cu_seqlens holds one entry more than there are sequences")
+    q, k, v = _rows(q, "q", 3, q), _rows(k, "k", 3, q), _rows(v, "v", 3, q)
+    y = _out(out, q)
+    T, H, D = q.shape
+    a = _lib.PromptArgs(_lib.dtype_code(q.dtype), cu.numel() - 1, T, H, k.shape[1], D,
+                        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                        v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), y.data_ptr(), y.stride(0), y.stride(1),
+                        float(D ** -0.5 if sm_scale is None else sm_scale), int(out is None))
+    _lib.launch("rb_prompt_attn", q, ctypes.byref(a))
+    return y
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=None, ahead=0, max_length=None, out=None):
+    """Attention of one new token per sequence over a paged KV cache.
+
+    q [B, H, 128]; k_pages, v_pages [pages, HK, page_size, 128]; table int32 [rows,
+    width] (page numbers, entries outside the pool name no page and their tokens are
+    left out), lengths int32 [rows]; seqs int32 [B]: the table row of each entry
+    (default: its own index). Entry b reads the first ``lengths + ahead`` tokens of its
+    row (``ahead`` counts tokens written but not committed yet), cut to the table's
+    width and to ``max_length``, a bound on the lengths that keeps scratch and launch
+    small when the table is much wider. No tokens give zeros. Returns [B, H, 128]."""
+    if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"paged_attention: q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)}, "
+                         f"v_pages {tuple(v_pages.shape)} do not fit")
+    _check_heads(q, k_pages.shape[1], k_pages.shape[3])
+    B, H, D = q.shape
+    table, lengths = _int32(table, "table", 2, q.device), _int32(lengths, "lengths", 1, q.device)
+    rows, width = table.shape
+    if lengths.numel() != rows:
+        raise ValueError(f"{lengths.numel()} lengths for {rows} table rows")
+    if seqs is None:
+        if rows != B:
+            raise ValueError(f"{rows} table rows for {B} queries: name the rows with seqs")
+    else:
+        seqs = _int32(seqs, "seqs", 1, q.device)
+        if seqs.numel() != B:
+            raise ValueError(f"{seqs.numel()} seqs for {B} queries")
+    if ahead < 0 or (max_length is not None and max_length < 1):
+        raise ValueError("ahead must not be negative, max_length must be positive")
+    q, k, v = _rows(q, "q", 3, q), _rows(k_pages, "k_pages", 4, q), _rows(v_pages, "v_pages", 4, q)
+    y = _out(out, q)
+    a = _lib.PagedArgs(_lib.dtype_code(q.dtype), B, H, k.shape[1], D, q.data_ptr(), q.stride(0), q.stride(1),
+                       k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                       v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k.shape[0], k.shape[2],
+                       table.data_ptr(), max(table.stride(0), width), width, rows, lengths.data_ptr(),
+                       seqs.data_ptr() if seqs is not None else None, int(ahead), int(max_length or 0),
+                       y.data_ptr(), y.stride(0), y.stride(1), float(D ** -0.5 if sm_scale is None else sm_scale))
+    nbytes = _lib.lib().rb_paged_attn_workspace(ctypes.byref(a))
+    ws = _lib.scratch(q, nbytes)
+    _lib.launch("rb_paged_attn", q, ctypes.byref(a), ws.data_ptr() if ws is not None else None, nbytes)
+    return y
