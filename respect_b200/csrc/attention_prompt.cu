@@ -69,11 +69,11 @@ __device__ __forceinline__ bool find_tile(const Dev& p, int tp, int rank, int* s
 
 // Rows before cu[0] and from cu[B] on belong to no sequence.
 template <typename T>
-__device__ __forceinline__ void zero_rest(const Dev& p) {
+__device__ __forceinline__ void zero_rest(const Dev& p, int threads) {   // the block's first `threads` threads
   const int a = start_of(p, 0), b = max(start_of(p, p.B), a);
   const int64_t n = static_cast<int64_t>(a + (p.T - b)) * p.H * kD;
-  for (int64_t x = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; x < n;
-       x += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * threads + threadIdx.x; x < n;
+       x += static_cast<int64_t>(gridDim.x) * threads) {
     int64_t t = x / (p.H * kD);
     if (t >= a) t += b - a;
     const int h = static_cast<int>(x / kD % p.H), d = static_cast<int>(x % kD);
@@ -157,19 +157,12 @@ __device__ __forceinline__ void mma3(float (&d)[4], const uint32_t (&ah)[4], con
 #pragma unroll
   for (int e = 0; e < 4; ++e) d[e] += t[e];
 }
-__device__ __forceinline__ float4 widen(const uint16_t* x) {
-  const uint2 u = *reinterpret_cast<const uint2*>(x);
-  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                     __uint_as_float(u.y & 0xFFFF0000u));
-}
-__device__ __forceinline__ float4 widen(const float* x) { return *reinterpret_cast<const float4*>(x); }
-__device__ __forceinline__ void copy16(float* dst, const void* src, uint32_t bytes) {
+__device__ __forceinline__ void copy16(float* dst, const float* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
 }  // namespace f32
 
-template <typename T>
-__global__ void __launch_bounds__(f32::kThreads) prompt_mma(const Dev p) {
+__global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
   using namespace f32;
   extern __shared__ __align__(16) float fsm[];
   float* Q = fsm;
@@ -177,7 +170,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_mma(const Dev p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   pdl_wait();
   pdl_trigger();
-  if (p.zero_rest) zero_rest<T>(p);
+  if (p.zero_rest) zero_rest<float>(p, kThreads);
   const int G = p.H / p.HK, TP = kRows / G;
   const int kvh = blockIdx.x % p.HK;
   int seq, tile;
@@ -185,29 +178,24 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_mma(const Dev p) {
   const int s0 = start_of(p, seq), len = length_of(p, seq);
   const int tok0 = tile * TP, toks = min(TP, len - tok0), rows = toks * G;
   const int tiles = (tok0 + toks + kKeys - 1) / kKeys;
-  const T* kg = static_cast<const T*>(p.k) + static_cast<int64_t>(s0) * p.skt + kvh * p.skh;
-  const T* vg = static_cast<const T*>(p.v) + static_cast<int64_t>(s0) * p.svt + kvh * p.svh;
+  const float* kg = static_cast<const float*>(p.k) + static_cast<int64_t>(s0) * p.skt + kvh * p.skh;
+  const float* vg = static_cast<const float*>(p.v) + static_cast<int64_t>(s0) * p.svt + kvh * p.svh;
   auto fetch = [&](int t) {   // rows past the sequence are zero
     float* K = KV + (t & 1) * 2 * kTile;
     for (int x = threadIdx.x; x < kKeys * 32; x += kThreads) {
       const int r = x >> 5, piece = (x & 31) * 4, key = t * kKeys + r;
       const bool ok = key < len;
-      if (sizeof(T) == 2) {   // bf16 widened: exact in one tf32 part
-        *reinterpret_cast<float4*>(K + r * kPitch + piece) = ok ? widen(kg + key * p.skt + piece) : make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<float4*>(K + kTile + r * kPitch + piece) = ok ? widen(vg + key * p.svt + piece) : make_float4(0.f, 0.f, 0.f, 0.f);
-        continue;
-      }
       copy16(K + r * kPitch + piece, ok ? kg + key * p.skt + piece : kg, ok ? 16u : 0u);
       copy16(K + kTile + r * kPitch + piece, ok ? vg + key * p.svt + piece : vg, ok ? 16u : 0u);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   fetch(0);
-  const T* qg = static_cast<const T*>(p.q) + static_cast<int64_t>(s0 + tok0) * p.sqt + kvh * G * p.sqh;
+  const float* qg = static_cast<const float*>(p.q) + static_cast<int64_t>(s0 + tok0) * p.sqt + kvh * G * p.sqh;
   for (int x = threadIdx.x; x < kRows * 32; x += kThreads) {
     const int r = x >> 5, piece = (x & 31) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < rows) v = widen(qg + r / G * p.sqt + r % G * p.sqh + piece);
+    if (r < rows) v = *reinterpret_cast<const float4*>(qg + r / G * p.sqt + r % G * p.sqh + piece);
     *reinterpret_cast<float4*>(Q + r * kPitch + piece) = v;
   }
   float o[kD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -305,21 +293,401 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_mma(const Dev p) {
     const int r = row0 + h * 8;
     bool nan = false;
     if (r < rows) {   // every row attends to itself: s >= 1, or NaN
-      T* out = static_cast<T*>(p.out) + static_cast<int64_t>(s0 + tok0 + r / G) * p.sot + (kvh * G + r % G) * p.soh;
+      float* out = static_cast<float*>(p.out) + static_cast<int64_t>(s0 + tok0 + r / G) * p.sot + (kvh * G + r % G) * p.soh;
 #pragma unroll
       for (int n = 0; n < kD / 8; ++n) {
         const float2 y = make_float2(o[n][h * 2] / s, o[n][h * 2 + 1] / s);
         nan |= y.x != y.x || y.y != y.y;
-        if (sizeof(T) == 4) *reinterpret_cast<float2*>(out + n * 8 + c * 2) = y;
-        else *reinterpret_cast<uint32_t*>(out + n * 8 + c * 2) = pack_bf16x2(y.x, y.y);
+        *reinterpret_cast<float2*>(out + n * 8 + c * 2) = y;
       }
     }
     unsigned again = __ballot_sync(0xffffffffu, nan);
     for (int x = 0; again; ++x, again >>= 4)
       if (again & 0xFu) {   // the four lanes of row x
         const int rr = warp * 16 + h * 8 + x;
-        redo_row<T>(p, s0, tok0 + rr / G, kvh * G + rr % G);
+        redo_row<float>(p, s0, tok0 + rr / G, kvh * G + rr % G);
       }
+  }
+}
+
+// ---------------------------------------------------------------- bf16
+// tcgen05. A block works on two tiles (A, B) of 128 rows, consecutive in the same
+// sequence and kv head, against K / V tiles of 128 keys: while the tensor core runs one
+// tile's products, the other tile's softmax runs, one thread per row.
+//
+//   S_t = Q_t K^T           tcgen05.mma 128 x 128 x 128 -> TMEM
+//   p = 2^(S scale2 - m)    m moves (and O, l are rescaled) only when the tile's maximum
+//                           exceeds it by more than 2^8: exact, and rare after the first tiles
+//   O_t += bf16(p) V        tcgen05.mma, A = P in tensor memory (over S_t), O stays in TMEM
+//
+// Warps 0-3 / 4-7: softmax of tile A / B, one row a thread (no exchange between
+// threads); warp 8: TMA (Q of the block, a ring of K and V tiles); warp 9: issues the
+// MMAs. The block is persistent: K / V and Q of its next work item arrive, and S of it
+// is computed, while the results of the last one are written out.
+namespace tcp {
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kHalf = 128 * 64 * 2;              // 64 dims of 128 rows: 16 KB, 128-byte swizzle
+constexpr int kTile = 2 * kHalf;
+constexpr int kRing = 5;                         // K / V buffers
+constexpr int kKVOff = 2 * kTile;                // after Q_A, Q_B
+constexpr int kBarOff = kKVOff + kRing * kTile;
+constexpr int kSmem = 1024 + kBarOff + 256;
+static_assert(kSmem <= 232448, "shared memory budget");
+constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last warpgroup: TMA, MMA and two idle warps
+// registers a thread: 168 at launch (3 x 128 of them); the softmax warps take what the others leave
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "register split");
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + kRing, S_FULL = KV_EMPTY + kRing, P_FULL = S_FULL + 2,
+       O_FULL = P_FULL + 2, NBAR = O_FULL + 2 };
+constexpr uint32_t kSCol = 0, kOCol = 256;       // S_t (and P_t) at 128 t, O_t at 256 + 128 t
+constexpr uint32_t kIdescQK = idesc_bf16_f32(128, 128, 0, 0);
+constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, 0, 1);
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_plain(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// 32 consecutive columns per thread, without the wait.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// One work item: two tiles of one sequence and kv head.
+struct Item {
+  int s0, len, tok0, kvh;   // sequence start, its length, first token of tile A
+  int n[2];                 // K / V tiles of A and B (0: the tile has no token)
+};
+__device__ __forceinline__ bool item_of(const Dev& p, int unit, Item* it) {
+  const int TP = kRows / (p.H / p.HK);
+  int seq, tile;
+  if (!find_tile(p, 2 * TP, unit / p.HK, &seq, &tile)) return false;
+  it->kvh = unit % p.HK;
+  it->s0 = start_of(p, seq);
+  it->len = length_of(p, seq);
+  it->tok0 = tile * 2 * TP;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = it->tok0 + t * TP, last = min(first + TP, it->len);   // one past the tile's last token
+    it->n[t] = first < it->len ? (last + kKeys - 1) / kKeys : 0;
+  }
+  return true;
+}
+}  // namespace tcp
+
+__global__ void __launch_bounds__(tcp::kThreads, 1)
+    prompt_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+              const __grid_constant__ CUtensorMap tv, const Dev p) {
+  using namespace tcp;
+  extern __shared__ uint8_t psm[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(psm) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBAR);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.H / p.HK, TP = kRows / G;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tq);
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    mbar_init(bar(Q_FULL), 1);
+    mbar_init(bar(Q_EMPTY), 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(bar(KV_FULL + i), 1);
+      mbar_init(bar(KV_EMPTY + i), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar(S_FULL + t), 1);
+      mbar_init(bar(P_FULL + t), kTileThreads);
+      mbar_init(bar(O_FULL + t), 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + kKVOff);
+  Item it;
+
+  if (warp >= kProducerWarp) {   // one setmaxnreg for the whole warpgroup
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kProducerWarp) {
+      uint32_t ring = 0;   // K / V tiles loaded so far
+      bool ok = true;
+      for (int unit = blockIdx.x, i = 0; ok && item_of(p, unit, &it); unit += gridDim.x, ++i) {
+        if (lane == 0) {
+          if (i > 0) ok = mbar_wait(bar(Q_EMPTY), (i - 1) & 1, 0x311);
+          if (ok) {
+            const int tiles = it.n[1] > 0 ? 2 : 1;
+            mbar_arrive_expect_tx(bar(Q_FULL), tiles * 2 * TP * G * 128);
+            for (int t = 0; t < tiles; ++t)
+              for (int h = 0; h < 2; ++h)
+                tma_load_4d(sQ + t * kTile + h * kHalf, &tq, bar(Q_FULL), h * 64, 0, it.kvh, it.s0 + it.tok0 + t * TP);
+          }
+          const int n = max(it.n[0], it.n[1]);
+          for (int x = 0; ok && x < 2 * n; ++x, ++ring) {   // K0, V0, K1, V1, ...
+            const int b = ring % kRing;
+            const uint32_t use = ring / kRing;
+            if (use > 0) ok = mbar_wait(bar(KV_EMPTY + b), (use - 1) & 1, 0x312);
+            if (!ok) break;
+            mbar_arrive_expect_tx(bar(KV_FULL + b), kTile);
+            const CUtensorMap* m = (x & 1) ? &tv : &tk;
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d_plain(sKV + b * kTile + h * kHalf, m, bar(KV_FULL + b), h * 64, it.s0 + (x >> 1) * kKeys, it.kvh);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+    } else if (warp == kMmaWarp) {
+      uint32_t ring = 0, steps[2] = {0, 0};   // steps[t]: P tiles of t consumed so far
+      bool ok = true;
+      for (int unit = blockIdx.x, i = 0; ok && item_of(p, unit, &it); unit += gridDim.x, ++i) {
+        if (lane == 0) {
+          const int n = max(it.n[0], it.n[1]);
+          auto full = [&](uint32_t r) { return mbar_wait(bar(KV_FULL + r % kRing), (r / kRing) & 1, 0x313); };
+          auto issue_s = [&](int t, uint32_t r) {
+            // a descriptor counts addresses in 16-byte units from bit 0: steps are plain additions
+            const uint64_t q = sdesc_kmajor_sw128(sQ + t * kTile), k = sdesc_kmajor_sw128(sKV + (r % kRing) * kTile);
+  #pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
+              umma_bf16(tmem + kSCol + t * 128, q + off, k + off, kIdescQK, kk ? 1u : 0u);
+            }
+            umma_commit(bar(S_FULL + t));
+          };
+          ok = mbar_wait(bar(Q_FULL), i & 1, 0x314) && full(ring);
+          if (ok) {
+            tc_fence_after();
+            issue_s(0, ring);
+            if (it.n[1] > 0) issue_s(1, ring);
+            umma_commit(bar(KV_EMPTY + ring % kRing));
+            if (n == 1) umma_commit(bar(Q_EMPTY));
+          }
+          for (int j = 0; ok && j < n; ++j) {   // V_j is ring + 1, K_{j + 1} ring + 2
+            ok = full(ring + 1);
+  #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || j >= it.n[t]) continue;
+              ok = mbar_wait(bar(P_FULL + t), steps[t] & 1, 0x315);
+              if (!ok) continue;
+              ++steps[t];
+              tc_fence_after();
+              const uint64_t v = sdesc_mnmajor_sw128(sKV + ((ring + 1) % kRing) * kTile, kHalf);
+  #pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+                umma_bf16_ta(tmem + kOCol + t * 128, tmem + kSCol + t * 128 + kk * 8, v + kk * (2048 >> 4), kIdescPV, (j | kk) ? 1u : 0u);
+              umma_commit(bar(O_FULL + t));
+              if (t == 1 || j >= it.n[1]) umma_commit(bar(KV_EMPTY + (ring + 1) % kRing));
+              if (j + 1 < it.n[t]) {
+                ok = full(ring + 2);
+                if (!ok) continue;
+                tc_fence_after();
+                issue_s(t, ring + 2);
+              }
+            }
+            if (ok && j + 1 < n) umma_commit(bar(KV_EMPTY + (ring + 2) % kRing));
+            if (ok && j + 2 == n) umma_commit(bar(Q_EMPTY));
+            ring += 2;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2, q4 = warp & 3;
+    const int r = q4 * 32 + lane;                      // row of the tile
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    const uint32_t st = lane_base + kSCol + t * 128, ot = lane_base + kOCol + t * 128;
+    const bool flip = p.scale2 < 0.f;                  // the largest weight is then at the smallest S
+    const float masked = flip ? INFINITY : -INFINITY;
+    const uint64_t scale_pair = pair(p.scale2, p.scale2);
+    uint32_t step = 0;                                 // S tiles consumed so far
+    uint32_t v_ring = 0;                               // ring number of the item's V_0, less one
+    bool ok = true;
+    bool more = item_of(p, blockIdx.x, &it);
+    for (int unit = blockIdx.x; ok && more;) {
+      const int n = it.n[t], N = max(it.n[0], it.n[1]);
+      const int tok = it.tok0 + t * TP + r / G;        // keys <= tok are attended
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++step) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(S_FULL + t), step & 1, 0x316));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(st + c * 32, s + c * 32);
+        tmem_wait_ld();
+        const int last = tok - j * kKeys;              // the last key of this tile that the row attends to
+        if (__any_sync(0xffffffffu, last < kKeys - 1)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c > last) s[c] = __float_as_uint(masked);
+        }
+        float top;
+        if (!flip) {
+          float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]), c = __uint_as_float(s[2]), d = __uint_as_float(s[3]);
+#pragma unroll
+          for (int x = 4; x < 128; x += 8) {
+            a = fmaxf(a, fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 1])));
+            b = fmaxf(b, fmaxf(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])));
+            if (x + 4 < 128) {
+              c = fmaxf(c, fmaxf(__uint_as_float(s[x + 4]), __uint_as_float(s[x + 5])));
+              d = fmaxf(d, fmaxf(__uint_as_float(s[x + 6]), __uint_as_float(s[x + 7])));
+            }
+          }
+          top = fmaxf(fmaxf(a, b), fmaxf(c, d));
+        } else {
+          top = __uint_as_float(s[0]);
+#pragma unroll
+          for (int x = 1; x < 128; ++x) top = fminf(top, __uint_as_float(s[x]));
+        }
+        top *= p.scale2;
+        const float m_new = top > m + kSlack ? top : m;
+        const float neg = m_new == -INFINITY ? 0.f : -m_new;
+        if (j > 0 && __any_sync(0xffffffffu, m_new != m)) {   // O of this warp's rows, once P V of the last tile is in
+          const float alpha = fast_exp2(m + neg);             // 1 for a row whose maximum stays
+          l *= alpha;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(O_FULL + t), (step - 1) & 1, 0x317));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16_nowait(ot + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(ot + c * 16, o);
+          }
+        }
+        m = m_new;
+        const uint64_t neg_pair = pair(neg, neg);
+        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint64_t x = fma2(pair(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1])), scale_pair, neg_pair);
+            float a, b;
+            unpair(x, a, b);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
+            sum[e & 1] = add2(sum[e & 1], pair(a, b));
+            w[e] = pack_bf16x2(a, b);
+          }
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(st + c * 8), "r"(w[0]),
+                       "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                       : "memory");
+        }
+        float a, b;
+        unpair(add2(sum[0], sum[1]), a, b);
+        l += a + b;
+        if ((j + 1) * kKeys > it.len && (t == 0 || j >= it.n[0])) {
+          // V rows past the sequence are another's: zero weights would not silence what they
+          // hold. The first tile to use this V clears them before its P V is issued.
+          const uint32_t ring = v_ring + 2 * j + 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(KV_FULL + ring % kRing), (ring / kRing) & 1, 0x318));
+          if (!ok) break;
+          uint8_t* v = smem + kKVOff + (ring % kRing) * kTile;
+          const int row = r;
+          if (j * kKeys + row >= it.len) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              *reinterpret_cast<uint4*>(v + row * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + kHalf + row * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(P_FULL + t));
+      }
+      const int s0 = it.s0, tok_end = min(it.tok0 + (t + 1) * TP, it.len), kvh = it.kvh;
+      unit += gridDim.x;
+      v_ring += 2 * N;
+      more = item_of(p, unit, &it);                    // while the last P V runs
+      if (n > 0 && ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(O_FULL + t), (step - 1) & 1, 0x319));
+        if (!ok) break;
+        tc_fence_after();
+        const bool live = r < TP * G && tok < tok_end;
+        const int h = kvh * G + r % G;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(s0 + tok) * p.sot + h * p.soh;
+        bool nan = false;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(ot + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float a = __uint_as_float(o[e * 8 + 2 * x]) / l, b = __uint_as_float(o[e * 8 + 2 * x + 1]) / l;
+              nan |= a != a || b != b;
+              w[x] = pack_bf16x2(a, b);
+            }
+            if (live) *reinterpret_cast<uint4*>(out + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        tc_fence_before();   // O read before the next item's P (and so its P V) is announced
+        for (unsigned again = __ballot_sync(0xffffffffu, nan && live); again; again &= again - 1) {
+          const int rr = q4 * 32 + __ffs(again) - 1;
+          redo_row<uint16_t>(p, s0, tok - r / G + rr / G, kvh * G + rr % G);
+        }
+      }
+    }
+    if (p.zero_rest) zero_rest<uint16_t>(p, 2 * kTileThreads);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -345,13 +713,34 @@ int prompt_launch(const rb_prompt_args* a, cudaStream_t st) {
   if (r != RB_OK || a->T == 0) return r;
   Dev p{a->q, a->k, a->v, a->sqt, a->sqh, a->skt, a->skh, a->svt, a->svh, a->cu, a->B, a->T, a->H, a->HK,
         a->out, a->sot, a->soh, a->sm_scale * 1.4426950408889634f, a->zero_rest};
-  const int TP = f32::kRows / (a->H / a->HK);
+  const int G = a->H / a->HK;
+  if (a->dtype == RB_BF16) {
+    if (a->sm_scale == 0.f) p.scale2 = 1e-37f;   // equal weights; a factor of zero would turn the mask's infinity into a NaN
+    const int TP = tcp::kRows / G;
+    const int64_t units = (static_cast<int64_t>(a->T) / (2 * TP) + a->B + 1) * a->HK;   // at most
+    if (units > INT32_MAX / 2) return RB_ERR_CAPACITY;
+    // a dimension of one entry may have any stride: give the map a plain one
+    const int64_t sqt = a->T > 1 ? a->sqt : 8, sqh = G > 1 ? a->sqh : 8, sqg = a->HK > 1 ? G * a->sqh : 8;
+    const int64_t skt = a->T > 1 ? a->skt : 8, skh = a->HK > 1 ? a->skh : 8, svt = a->T > 1 ? a->svt : 8, svh = a->HK > 1 ? a->svh : 8;
+    CUtensorMap tq, tk, tv;
+    const uint64_t dims[4] = {kD, static_cast<uint64_t>(G), static_cast<uint64_t>(a->HK), static_cast<uint64_t>(a->T)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(sqh) * 2, static_cast<uint64_t>(sqg) * 2, static_cast<uint64_t>(sqt) * 2};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TP)};
+    r = encode_tiled(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, a->q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r == RB_OK) r = encode_heads_3d(&tk, a->k, a->T, a->HK, skt, skh);
+    if (r == RB_OK) r = encode_heads_3d(&tv, a->v, a->T, a->HK, svt, svh);
+    if (r != RB_OK) return r;
+    if (cudaFuncSetAttribute(prompt_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, tcp::kSmem) != cudaSuccess)
+      return RB_ERR_CUDA;
+    const int64_t grid = units < device_sm_count() ? units : device_sm_count();
+    return launch_k(prompt_tc, dim3(static_cast<unsigned>(grid)), dim3(tcp::kThreads), tcp::kSmem, st, true, tq, tk, tv, p);
+  }
+  const int TP = f32::kRows / G;
   const int64_t grid = (static_cast<int64_t>(a->T) / TP + a->B + 1) * a->HK;   // tiles at most
   if (grid > INT32_MAX) return RB_ERR_CAPACITY;
-  const auto kern = a->dtype == RB_F32 ? prompt_mma<float> : prompt_mma<uint16_t>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, f32::kSmem) != cudaSuccess)
+  if (cudaFuncSetAttribute(prompt_f32, cudaFuncAttributeMaxDynamicSharedMemorySize, f32::kSmem) != cudaSuccess)
     return RB_ERR_CUDA;
-  return launch_k(kern, dim3(static_cast<unsigned>(grid)), dim3(f32::kThreads), f32::kSmem, st, true, p);
+  return launch_k(prompt_f32, dim3(static_cast<unsigned>(grid)), dim3(f32::kThreads), f32::kSmem, st, true, p);
 }
 
 }  // namespace rb
