@@ -7,8 +7,7 @@
 // fill the rows. Keys are taken in tiles at absolute positions of the sequence, in
 // ascending order; a tile that lies wholly after a row's token changes nothing of
 // that row. A row's bits therefore depend on its own sequence alone, not on the
-// packing or on which tile it falls into. Tiles are handed out heaviest first (by
-// their number within the sequence), so that the last blocks to run are short.
+// packing or on which tile it falls into.
 #include "common.cuh"
 #include "host_util.h"
 
@@ -25,44 +24,53 @@ struct Dev {
   void* out;
   int64_t sot, soh;
   float scale2;                            // sm_scale * log2 e
+  int wide;                                // tiles of a band: about as many as run at a time
   int zero_rest;                           // rows of no sequence: zeros (else left alone)
 };
 
 __device__ __forceinline__ int start_of(const Dev& p, int i) { return min(max(p.cu[i], 0), p.T); }
 __device__ __forceinline__ int length_of(const Dev& p, int i) { return max(start_of(p, i + 1) - start_of(p, i), 0); }
 
-// The rank-th tile of tp tokens in descending order of its number within its
-// sequence (the earlier sequence first among equals). Warp-wide, the same in every
-// lane; false when there are fewer tiles. `above(L)` counts the tiles numbered >= L.
-__device__ __forceinline__ bool find_tile(const Dev& p, int tp, int rank, int* seq, int* tile) {
+// The rank-th tile of tp tokens. Tiles are ordered by the band of `wide` tiles they lie
+// in, the later band first, then by sequence, then the later tile first: work falls
+// from the first rank to the last, and tiles that run at the same time read the same
+// K / V. Warp-wide, the same in every lane; false when there are fewer tiles.
+__device__ __forceinline__ bool find_tile(const Dev& p, int tp, int wide, int rank, int* seq, int* tile) {
   const int lane = threadIdx.x & 31;
   int tiles0 = 0, most = 0;   // this lane's first sequence is looked at often
   if (lane < p.B) tiles0 = (length_of(p, lane) + tp - 1) / tp;
   for (int i = lane; i < p.B; i += 32) most = max(most, i == lane ? tiles0 : (length_of(p, i) + tp - 1) / tp);
-  most = __reduce_max_sync(0xffffffffu, most);
-  auto above = [&](int L) {
-    int n = max(tiles0 - L, 0);
-    for (int i = lane + 32; i < p.B; i += 32) n += max((length_of(p, i) + tp - 1) / tp - L, 0);
+  most = (__reduce_max_sync(0xffffffffu, most) + wide - 1) / wide;   // bands
+  auto from = [&](int band) {                                        // tiles in it and in later ones
+    int n = max(tiles0 - band * wide, 0);
+    for (int i = lane + 32; i < p.B; i += 32) n += max((length_of(p, i) + tp - 1) / tp - band * wide, 0);
     return __reduce_add_sync(0xffffffffu, n);
   };
-  if (above(0) <= rank) return false;
-  int lo = 0, hi = most;      // above(lo) > rank >= above(hi)
+  if (from(0) <= rank) return false;
+  int lo = 0, hi = most;      // from(lo) > rank >= from(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (above(mid) > rank) lo = mid; else hi = mid;
+    if (from(mid) > rank) lo = mid; else hi = mid;
   }
-  int left = rank - above(lo + 1);   // among the sequences with more than lo tiles
+  int left = rank - from(lo + 1);   // within the band
   for (int base = 0; base < p.B; base += 32) {
     const int i = base + lane;
     const int n = base == 0 ? tiles0 : i < p.B ? (length_of(p, i) + tp - 1) / tp : 0;
-    const unsigned has = __ballot_sync(0xffffffffu, n > lo);
-    const int c = __popc(has);
-    if (left < c) {
-      *seq = base + __fns(has, 0, left + 1);
-      *tile = lo;
+    const int here = min(max(n - lo * wide, 0), wide);
+    int sum = here;           // inclusive prefix sum
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, sum > left);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      *seq = base + l;
+      *tile = lo * wide + __shfl_sync(0xffffffffu, sum, l) - 1 - left;
       return true;
     }
-    left -= c;
+    left -= __shfl_sync(0xffffffffu, sum, 31);
   }
   return false;
 }
@@ -174,7 +182,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
   const int G = p.H / p.HK, TP = kRows / G;
   const int kvh = blockIdx.x % p.HK;
   int seq, tile;
-  if (!find_tile(p, TP, blockIdx.x / p.HK, &seq, &tile)) return;
+  if (!find_tile(p, TP, p.wide, blockIdx.x / p.HK, &seq, &tile)) return;
   const int s0 = start_of(p, seq), len = length_of(p, seq);
   const int tok0 = tile * TP, toks = min(TP, len - tok0), rows = toks * G;
   const int tiles = (tok0 + toks + kKeys - 1) / kKeys;
@@ -331,15 +339,18 @@ constexpr int kTile = 2 * kHalf;
 constexpr int kRing = 5;                         // K / V buffers
 constexpr int kKVOff = 2 * kTile;                // after Q_A, Q_B
 constexpr int kBarOff = kKVOff + kRing * kTile;
-constexpr int kSmem = 1024 + kBarOff + 256;
+constexpr int kItemOff = kBarOff + 256;          // announced items, 32 bytes each
+constexpr int kSmem = 1024 + kItemOff + 64;
 static_assert(kSmem <= 232448, "shared memory budget");
-constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last warpgroup: TMA, MMA and two idle warps
+constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last warpgroup: TMA, MMA, the work items, an idle warp
 // registers a thread: 168 at launch (3 x 128 of them); the softmax warps take what the others leave
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "register split");
-constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kItemWarp = 10;
+constexpr int kParts = 2;                        // P is handed over in parts of 64 keys
+constexpr int kItems = 2;                        // work items announced ahead
 enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + kRing, S_FULL = KV_EMPTY + kRing, P_FULL = S_FULL + 2,
-       O_FULL = P_FULL + 2, NBAR = O_FULL + 2 };
+       O_FULL = P_FULL + 2 * kParts, ITEM_FULL = O_FULL + 2, ITEM_EMPTY = ITEM_FULL + kItems, NBAR = ITEM_EMPTY + kItems };
 constexpr uint32_t kSCol = 0, kOCol = 256;       // S_t (and P_t) at 128 t, O_t at 256 + 128 t
 constexpr uint32_t kIdescQK = idesc_bf16_f32(128, 128, 0, 0);
 constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, 0, 1);
@@ -385,15 +396,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// The i-th work item of a block: the blocks take turns forwards and backwards, so that
+// a round's heavy end does not always fall to the same block.
+__device__ __forceinline__ int unit_of(int i) {
+  return i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // One work item: two tiles of one sequence and kv head.
 struct Item {
   int s0, len, tok0, kvh;   // sequence start, its length, first token of tile A
-  int n[2];                 // K / V tiles of A and B (0: the tile has no token)
+  int n[2];                 // K / V tiles of A and B (0: the tile has no token; A has one, or there is no item)
+  int pad[2];
 };
-__device__ __forceinline__ bool item_of(const Dev& p, int unit, Item* it) {
+__device__ __forceinline__ void item_of(const Dev& p, int unit, Item* it) {
   const int TP = kRows / (p.H / p.HK);
   int seq, tile;
-  if (!find_tile(p, 2 * TP, unit / p.HK, &seq, &tile)) return false;
+  it->n[0] = 0;
+  if (!find_tile(p, 2 * TP, p.wide, unit / p.HK, &seq, &tile)) return;
   it->kvh = unit % p.HK;
   it->s0 = start_of(p, seq);
   it->len = length_of(p, seq);
@@ -403,7 +422,6 @@ __device__ __forceinline__ bool item_of(const Dev& p, int unit, Item* it) {
     const int first = it->tok0 + t * TP, last = min(first + TP, it->len);   // one past the tile's last token
     it->n[t] = first < it->len ? (last + kKeys - 1) / kKeys : 0;
   }
-  return true;
 }
 }  // namespace tcp
 
@@ -431,8 +449,12 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar(S_FULL + t), 1);
-      mbar_init(bar(P_FULL + t), kTileThreads);
+      for (int x = 0; x < kParts; ++x) mbar_init(bar(P_FULL + t * kParts + x), kTileThreads);
       mbar_init(bar(O_FULL + t), 1);
+    }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(bar(ITEM_FULL + i), 1);
+      mbar_init(bar(ITEM_EMPTY + i), 10);   // eight softmax warps, TMA, MMA
     }
     fence_mbar_init();
   }
@@ -447,14 +469,24 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   pdl_wait();
   pdl_trigger();
   const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + kKVOff);
+  Item* items = reinterpret_cast<Item*>(smem + kItemOff);
   Item it;
+  // The i-th item, as announced; false after the last one (or after a wait gave up).
+  auto next_item = [&](int i) {
+    const int x = i % kItems;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar(ITEM_FULL + x), (i / kItems) & 1, 0x31a))) return false;
+    it = items[x];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + x));
+    return it.n[0] > 0;
+  };
 
   if (warp >= kProducerWarp) {   // one setmaxnreg for the whole warpgroup
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kProducerWarp) {
       uint32_t ring = 0;   // K / V tiles loaded so far
       bool ok = true;
-      for (int unit = blockIdx.x, i = 0; ok && item_of(p, unit, &it); unit += gridDim.x, ++i) {
+      for (int i = 0; ok && next_item(i); ++i) {
         if (lane == 0) {
           if (i > 0) ok = mbar_wait(bar(Q_EMPTY), (i - 1) & 1, 0x311);
           if (ok) {
@@ -481,7 +513,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     } else if (warp == kMmaWarp) {
       uint32_t ring = 0, steps[2] = {0, 0};   // steps[t]: P tiles of t consumed so far
       bool ok = true;
-      for (int unit = blockIdx.x, i = 0; ok && item_of(p, unit, &it); unit += gridDim.x, ++i) {
+      for (int i = 0; ok && next_item(i); ++i) {
         if (lane == 0) {
           const int n = max(it.n[0], it.n[1]);
           auto full = [&](uint32_t r) { return mbar_wait(bar(KV_FULL + r % kRing), (r / kRing) & 1, 0x313); };
@@ -508,14 +540,21 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   #pragma unroll
             for (int t = 0; t < 2; ++t) {
               if (!ok || j >= it.n[t]) continue;
-              ok = mbar_wait(bar(P_FULL + t), steps[t] & 1, 0x315);
+              ok = mbar_wait(bar(P_FULL + t * kParts), steps[t] & 1, 0x315);
               if (!ok) continue;
-              ++steps[t];
               tc_fence_after();
               const uint64_t v = sdesc_mnmajor_sw128(sKV + ((ring + 1) % kRing) * kTile, kHalf);
   #pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)
-                umma_bf16_ta(tmem + kOCol + t * 128, tmem + kSCol + t * 128 + kk * 8, v + kk * (2048 >> 4), kIdescPV, (j | kk) ? 1u : 0u);
+              for (int kk = 0; kk < kKeys / 16; ++kk) {
+                if (kk == kKeys / 16 / kParts) {
+                  ok = mbar_wait(bar(P_FULL + t * kParts + 1), steps[t] & 1, 0x31b);
+                  tc_fence_after();
+                }
+                if (ok)
+                  umma_bf16_ta(tmem + kOCol + t * 128, tmem + kSCol + t * 128 + kk * 8, v + kk * (2048 >> 4), kIdescPV, (j | kk) ? 1u : 0u);
+              }
+              if (!ok) continue;
+              ++steps[t];
               umma_commit(bar(O_FULL + t));
               if (t == 1 || j >= it.n[1]) umma_commit(bar(KV_EMPTY + (ring + 1) % kRing));
               if (j + 1 < it.n[t]) {
@@ -532,6 +571,19 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
+    } else if (warp == kItemWarp) {
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        item_of(p, unit_of(i), &it);
+        const int x = i % kItems;
+        if (i >= kItems) ok = __all_sync(0xffffffffu, mbar_wait(bar(ITEM_EMPTY + x), ((i / kItems) - 1) & 1, 0x31c));
+        if (!ok) break;
+        if (lane == 0) {
+          items[x] = it;
+          mbar_arrive(bar(ITEM_FULL + x));
+        }
+        if (it.n[0] == 0) break;
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -545,8 +597,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     uint32_t step = 0;                                 // S tiles consumed so far
     uint32_t v_ring = 0;                               // ring number of the item's V_0, less one
     bool ok = true;
-    bool more = item_of(p, blockIdx.x, &it);
-    for (int unit = blockIdx.x; ok && more;) {
+    for (int i = 0; ok && next_item(i); ++i) {
       const int n = it.n[t], N = max(it.n[0], it.n[1]);
       const int tok = it.tok0 + t * TP + r / G;        // keys <= tok are attended
       float m = -INFINITY, l = 0.f;
@@ -602,28 +653,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           }
         }
         m = m_new;
-        const uint64_t neg_pair = pair(neg, neg);
-        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint64_t x = fma2(pair(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1])), scale_pair, neg_pair);
-            float a, b;
-            unpair(x, a, b);
-            a = fast_exp2(a);
-            b = fast_exp2(b);
-            sum[e & 1] = add2(sum[e & 1], pair(a, b));
-            w[e] = pack_bf16x2(a, b);
-          }
-          asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(st + c * 8), "r"(w[0]),
-                       "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                       : "memory");
-        }
-        float a, b;
-        unpair(add2(sum[0], sum[1]), a, b);
-        l += a + b;
         if ((j + 1) * kKeys > it.len && (t == 0 || j >= it.n[0])) {
           // V rows past the sequence are another's: zero weights would not silence what they
           // hold. The first tile to use this V clears them before its P V is issued.
@@ -631,31 +660,51 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           ok = __all_sync(0xffffffffu, mbar_wait(bar(KV_FULL + ring % kRing), (ring / kRing) & 1, 0x318));
           if (!ok) break;
           uint8_t* v = smem + kKVOff + (ring % kRing) * kTile;
-          const int row = r;
-          if (j * kKeys + row >= it.len) {
+          if (j * kKeys + r >= it.len) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-              *reinterpret_cast<uint4*>(v + row * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(v + kHalf + row * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + r * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + kHalf + r * 128 + x * 16) = make_uint4(0, 0, 0, 0);
             }
           }
           fence_proxy_async_smem();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(bar(P_FULL + t));
+        const uint64_t neg_pair = pair(neg, neg);
+        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t x = fma2(pair(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])), scale_pair, neg_pair);
+            float a, b;
+            unpair(x, a, b);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
+            sum[e & 1] = add2(sum[e & 1], pair(a, b));
+            w[e] = pack_bf16x2(a, b);
+          }
+          tmem_st16(st + c * 16, w);
+          if ((c + 1) % (4 / kParts) == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(P_FULL + t * kParts + c / (4 / kParts)));
+          }
+        }
+        float a, b;
+        unpair(add2(sum[0], sum[1]), a, b);
+        l += a + b;
       }
-      const int s0 = it.s0, tok_end = min(it.tok0 + (t + 1) * TP, it.len), kvh = it.kvh;
-      unit += gridDim.x;
+      const int tok_end = min(it.tok0 + (t + 1) * TP, it.len);
       v_ring += 2 * N;
-      more = item_of(p, unit, &it);                    // while the last P V runs
       if (n > 0 && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(O_FULL + t), (step - 1) & 1, 0x319));
         if (!ok) break;
         tc_fence_after();
         const bool live = r < TP * G && tok < tok_end;
-        const int h = kvh * G + r % G;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(s0 + tok) * p.sot + h * p.soh;
+        const int h = it.kvh * G + r % G;
+        uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(it.s0 + tok) * p.sot + h * p.soh;
+        const float inv = 1.f / l;
         bool nan = false;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -667,7 +716,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             uint32_t w[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const float a = __uint_as_float(o[e * 8 + 2 * x]) / l, b = __uint_as_float(o[e * 8 + 2 * x + 1]) / l;
+              const float a = __uint_as_float(o[e * 8 + 2 * x]) * inv, b = __uint_as_float(o[e * 8 + 2 * x + 1]) * inv;
               nan |= a != a || b != b;
               w[x] = pack_bf16x2(a, b);
             }
@@ -677,7 +726,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         tc_fence_before();   // O read before the next item's P (and so its P V) is announced
         for (unsigned again = __ballot_sync(0xffffffffu, nan && live); again; again &= again - 1) {
           const int rr = q4 * 32 + __ffs(again) - 1;
-          redo_row<uint16_t>(p, s0, tok - r / G + rr / G, kvh * G + rr % G);
+          redo_row<uint16_t>(p, it.s0, tok - r / G + rr / G, it.kvh * G + rr % G);
         }
       }
     }
@@ -712,7 +761,7 @@ int prompt_launch(const rb_prompt_args* a, cudaStream_t st) {
   int r = prompt_validate(a);
   if (r != RB_OK || a->T == 0) return r;
   Dev p{a->q, a->k, a->v, a->sqt, a->sqh, a->skt, a->skh, a->svt, a->svh, a->cu, a->B, a->T, a->H, a->HK,
-        a->out, a->sot, a->soh, a->sm_scale * 1.4426950408889634f, a->zero_rest};
+        a->out, a->sot, a->soh, a->sm_scale * 1.4426950408889634f, (device_sm_count() + a->HK - 1) / a->HK, a->zero_rest};
   const int G = a->H / a->HK;
   if (a->dtype == RB_BF16) {
     if (a->sm_scale == 0.f) p.scale2 = 1e-37f;   // equal weights; a factor of zero would turn the mask's infinity into a NaN
