@@ -396,10 +396,51 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ bool elect_one() {   // true in one lane of a converged warp
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // The i-th work item of a block: the blocks take turns forwards and backwards, so that
 // a round's heavy end does not always fall to the same block.
 __device__ __forceinline__ int unit_of(int i) {
   return i * gridDim.x + ((i & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
+// 2^x for a pair on the FMA pipe: x = n + f with n = round(x), |f| <= 1/2, times a cubic
+// for 2^f (least relative error with the constant fixed at 1, found numerically: 2^-13.3,
+// against the 2^-9 of the bf16 weight it becomes). x is at most kSlack; below -127, and
+// for a masked -inf, the result is exactly 0; a NaN stays one.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(b), "f"(-127.f));
+  x = pair(a, b);
+  constexpr float kShift = 12582912.f + 127.f;   // 1.5 * 2^23: the low bits of x + kShift are n + 127
+  const uint64_t t = add2(x, pair(kShift, kShift));
+  const uint64_t f = sub2(x, sub2(t, pair(kShift, kShift)));
+  uint64_t y = fma2(f, pair(0.05500892f, 0.05500892f), pair(0.24221096f, 0.24221096f));
+  y = fma2(y, f, pair(0.69328293f, 0.69328293f));
+  y = fma2(y, f, pair(1.f, 1.f));
+  unpair(t, a, b);
+  return mul2(y, pair(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
 }
 
 // One work item: two tiles of one sequence and kv head.
@@ -434,7 +475,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBAR);
   auto bar = [&](int i) { return smem_u32(bars + i); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = p.H / p.HK, TP = kRows / G;
 
   if (threadIdx.x == 0) {
@@ -449,7 +490,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar(S_FULL + t), 1);
-      for (int x = 0; x < kParts; ++x) mbar_init(bar(P_FULL + t * kParts + x), kTileThreads);
+      for (int x = 0; x < kParts; ++x) mbar_init(bar(P_FULL + t * kParts + x), kTileThreads / 32);
       mbar_init(bar(O_FULL + t), 1);
     }
     for (int i = 0; i < kItems; ++i) {
@@ -465,7 +506,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
   pdl_trigger();
   const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + kKVOff);
@@ -474,7 +515,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   // The i-th item, as announced; false after the last one (or after a wait gave up).
   auto next_item = [&](int i) {
     const int x = i % kItems;
-    if (!__all_sync(0xffffffffu, mbar_wait(bar(ITEM_FULL + x), (i / kItems) & 1, 0x31a))) return false;
+    if (!__all_sync(0xffffffffu, mbar_wait_spin(bar(ITEM_FULL + x), (i / kItems) & 1, 0x31a))) return false;
     it = items[x];
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(ITEM_EMPTY + x));
@@ -488,7 +529,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       bool ok = true;
       for (int i = 0; ok && next_item(i); ++i) {
         if (lane == 0) {
-          if (i > 0) ok = mbar_wait(bar(Q_EMPTY), (i - 1) & 1, 0x311);
+          if (i > 0) ok = mbar_wait_spin(bar(Q_EMPTY), (i - 1) & 1, 0x311);
           if (ok) {
             const int tiles = it.n[1] > 0 ? 2 : 1;
             mbar_arrive_expect_tx(bar(Q_FULL), tiles * 2 * TP * G * 128);
@@ -500,7 +541,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           for (int x = 0; ok && x < 2 * n; ++x, ++ring) {   // K0, V0, K1, V1, ...
             const int b = ring % kRing;
             const uint32_t use = ring / kRing;
-            if (use > 0) ok = mbar_wait(bar(KV_EMPTY + b), (use - 1) & 1, 0x312);
+            if (use > 0) ok = mbar_wait_spin(bar(KV_EMPTY + b), (use - 1) & 1, 0x312);
             if (!ok) break;
             mbar_arrive_expect_tx(bar(KV_FULL + b), kTile);
             const CUtensorMap* m = (x & 1) ? &tv : &tk;
@@ -511,72 +552,95 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
     } else if (warp == kMmaWarp) {
-      uint32_t ring = 0, steps[2] = {0, 0};   // steps[t]: P tiles of t consumed so far
+      // The whole warp keeps the books, one lane issues: its loop is nothing but MMAs with
+      // descriptors a constant apart (a branch or an address computation between them costs
+      // more than the 64 cycles an MMA takes). Descriptors count addresses in 16-byte units
+      // from bit 0, so steps are plain additions.
+      const bool leader = elect_one();
+      const uint64_t dq = sdesc_kmajor_sw128(sQ), dk = sdesc_kmajor_sw128(sKV), dv = sdesc_mnmajor_sw128(sKV, kHalf);
+      uint32_t buf = 0, phase = 0;        // of the next K / V tile
+      uint32_t steps[2] = {0, 0};         // P tiles of A and B consumed so far
+      auto advance = [&] {
+        if (++buf == kRing) {
+          buf = 0;
+          phase ^= 1;
+        }
+      };
+      auto issue_s = [&](int t, uint32_t kbuf) {
+        if (leader) {
+          const uint64_t q = dq + t * (kTile >> 4), k = dk + kbuf * (kTile >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
+            umma_bf16(tmem + kSCol + t * 128, q + off, k + off, kIdescQK, kk ? 1u : 0u);
+          }
+          umma_commit(bar(S_FULL + t));
+        }
+      };
+      auto issue_o = [&](int t, uint32_t vbuf, int part, uint32_t add) {
+        if (leader) {
+          const uint64_t v = dv + vbuf * (kTile >> 4) + part * (kKeys / 16 / kParts * (2048 >> 4));
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16 / kParts; ++kk)
+            umma_bf16_ta(tmem + kOCol + t * 128, tmem + kSCol + t * 128 + part * (64 / kParts) + kk * 8, v + kk * (2048 >> 4),
+                         kIdescPV, kk ? 1u : add);
+        }
+      };
+      auto commit = [&](int b) {
+        if (leader) umma_commit(bar(b));
+      };
       bool ok = true;
       for (int i = 0; ok && next_item(i); ++i) {
-        if (lane == 0) {
-          const int n = max(it.n[0], it.n[1]);
-          auto full = [&](uint32_t r) { return mbar_wait(bar(KV_FULL + r % kRing), (r / kRing) & 1, 0x313); };
-          auto issue_s = [&](int t, uint32_t r) {
-            // a descriptor counts addresses in 16-byte units from bit 0: steps are plain additions
-            const uint64_t q = sdesc_kmajor_sw128(sQ + t * kTile), k = sdesc_kmajor_sw128(sKV + (r % kRing) * kTile);
-  #pragma unroll
-            for (int kk = 0; kk < kD / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * kHalf + (kk & 3) * 32) >> 4;
-              umma_bf16(tmem + kSCol + t * 128, q + off, k + off, kIdescQK, kk ? 1u : 0u);
+        const int n = max(it.n[0], it.n[1]);
+        ok = mbar_wait_spin(bar(Q_FULL), i & 1, 0x314) && mbar_wait_spin(bar(KV_FULL + buf), phase, 0x313);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(0, buf);
+        if (it.n[1] > 0) issue_s(1, buf);
+        commit(KV_EMPTY + buf);
+        if (n == 1) commit(Q_EMPTY);
+        advance();
+        for (int j = 0; ok && j < n; ++j) {
+          const uint32_t vbuf = buf, vphase = phase;
+          advance();                      // buf, phase: K of the next tile, if there is one
+          const bool more = j + 1 < n;
+          bool v_in = false, k_in = false;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || j >= it.n[t]) continue;
+            if (!v_in) ok = v_in = mbar_wait_spin(bar(KV_FULL + vbuf), vphase, 0x313);
+#pragma unroll
+            for (int x = 0; x < kParts; ++x) {
+              ok = ok && mbar_wait_spin(bar(P_FULL + t * kParts + x), steps[t] & 1, 0x315);
+              if (!ok) break;
+              tc_fence_after();
+              issue_o(t, vbuf, x, (j | x) ? 1u : 0u);
             }
-            umma_commit(bar(S_FULL + t));
-          };
-          ok = mbar_wait(bar(Q_FULL), i & 1, 0x314) && full(ring);
-          if (ok) {
-            tc_fence_after();
-            issue_s(0, ring);
-            if (it.n[1] > 0) issue_s(1, ring);
-            umma_commit(bar(KV_EMPTY + ring % kRing));
-            if (n == 1) umma_commit(bar(Q_EMPTY));
-          }
-          for (int j = 0; ok && j < n; ++j) {   // V_j is ring + 1, K_{j + 1} ring + 2
-            ok = full(ring + 1);
-  #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!ok || j >= it.n[t]) continue;
-              ok = mbar_wait(bar(P_FULL + t * kParts), steps[t] & 1, 0x315);
+            if (!ok) continue;
+            ++steps[t];
+            commit(O_FULL + t);
+            if (t == 1 || j >= it.n[1]) commit(KV_EMPTY + vbuf);
+            if (j + 1 < it.n[t]) {
+              if (!k_in) ok = k_in = mbar_wait_spin(bar(KV_FULL + buf), phase, 0x31b);
               if (!ok) continue;
               tc_fence_after();
-              const uint64_t v = sdesc_mnmajor_sw128(sKV + ((ring + 1) % kRing) * kTile, kHalf);
-  #pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk) {
-                if (kk == kKeys / 16 / kParts) {
-                  ok = mbar_wait(bar(P_FULL + t * kParts + 1), steps[t] & 1, 0x31b);
-                  tc_fence_after();
-                }
-                if (ok)
-                  umma_bf16_ta(tmem + kOCol + t * 128, tmem + kSCol + t * 128 + kk * 8, v + kk * (2048 >> 4), kIdescPV, (j | kk) ? 1u : 0u);
-              }
-              if (!ok) continue;
-              ++steps[t];
-              umma_commit(bar(O_FULL + t));
-              if (t == 1 || j >= it.n[1]) umma_commit(bar(KV_EMPTY + (ring + 1) % kRing));
-              if (j + 1 < it.n[t]) {
-                ok = full(ring + 2);
-                if (!ok) continue;
-                tc_fence_after();
-                issue_s(t, ring + 2);
-              }
+              issue_s(t, buf);
             }
-            if (ok && j + 1 < n) umma_commit(bar(KV_EMPTY + (ring + 2) % kRing));
-            if (ok && j + 2 == n) umma_commit(bar(Q_EMPTY));
-            ring += 2;
+          }
+          if (ok && more) {
+            commit(KV_EMPTY + buf);
+            if (j + 2 == n) commit(Q_EMPTY);
+            advance();
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu, ok);
       }
     } else if (warp == kItemWarp) {
       bool ok = true;
       for (int i = 0; ok; ++i) {
         item_of(p, unit_of(i), &it);
         const int x = i % kItems;
-        if (i >= kItems) ok = __all_sync(0xffffffffu, mbar_wait(bar(ITEM_EMPTY + x), ((i / kItems) - 1) & 1, 0x31c));
+        if (i >= kItems) ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(ITEM_EMPTY + x), ((i / kItems) - 1) & 1, 0x31c));
         if (!ok) break;
         if (lane == 0) {
           items[x] = it;
@@ -602,7 +666,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       const int tok = it.tok0 + t * TP + r / G;        // keys <= tok are attended
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++step) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(S_FULL + t), step & 1, 0x316));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(bar(S_FULL + t), step & 1, 0x316));
         if (!ok) break;
         tc_fence_after();
         uint32_t s[128];
@@ -619,14 +683,14 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         if (!flip) {
           float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]), c = __uint_as_float(s[2]), d = __uint_as_float(s[3]);
 #pragma unroll
-          for (int x = 4; x < 128; x += 8) {
-            a = fmaxf(a, fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 1])));
-            b = fmaxf(b, fmaxf(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])));
-            if (x + 4 < 128) {
-              c = fmaxf(c, fmaxf(__uint_as_float(s[x + 4]), __uint_as_float(s[x + 5])));
-              d = fmaxf(d, fmaxf(__uint_as_float(s[x + 6]), __uint_as_float(s[x + 7])));
-            }
+          for (int x = 4; x < 124; x += 8) {
+            a = max3(a, __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
+            b = max3(b, __uint_as_float(s[x + 2]), __uint_as_float(s[x + 3]));
+            c = max3(c, __uint_as_float(s[x + 4]), __uint_as_float(s[x + 5]));
+            d = max3(d, __uint_as_float(s[x + 6]), __uint_as_float(s[x + 7]));
           }
+          a = max3(a, __uint_as_float(s[124]), __uint_as_float(s[125]));
+          b = max3(b, __uint_as_float(s[126]), __uint_as_float(s[127]));
           top = fmaxf(fmaxf(a, b), fmaxf(c, d));
         } else {
           top = __uint_as_float(s[0]);
@@ -639,7 +703,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         if (j > 0 && __any_sync(0xffffffffu, m_new != m)) {   // O of this warp's rows, once P V of the last tile is in
           const float alpha = fast_exp2(m + neg);             // 1 for a row whose maximum stays
           l *= alpha;
-          ok = __all_sync(0xffffffffu, mbar_wait(bar(O_FULL + t), (step - 1) & 1, 0x317));
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(O_FULL + t), (step - 1) & 1, 0x317));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -657,7 +721,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           // V rows past the sequence are another's: zero weights would not silence what they
           // hold. The first tile to use this V clears them before its P V is issued.
           const uint32_t ring = v_ring + 2 * j + 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(bar(KV_FULL + ring % kRing), (ring / kRing) & 1, 0x318));
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(KV_FULL + ring % kRing), (ring / kRing) & 1, 0x318));
           if (!ok) break;
           uint8_t* v = smem + kKVOff + (ring % kRing) * kTile;
           if (j * kKeys + r >= it.len) {
@@ -678,17 +742,25 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           for (int e = 0; e < 16; ++e) {
             const uint64_t x = fma2(pair(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])), scale_pair, neg_pair);
             float a, b;
-            unpair(x, a, b);
-            a = fast_exp2(a);
-            b = fast_exp2(b);
-            sum[e & 1] = add2(sum[e & 1], pair(a, b));
+            uint64_t y;
+            if (e % 4 == 3) {   // a quarter on the FMA pipe: 2^x on the other one is the longer queue
+              y = exp2_pair(x);
+              unpair(y, a, b);
+            } else {
+              unpair(x, a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              y = pair(a, b);
+            }
+            sum[e & 1] = add2(sum[e & 1], y);
             w[e] = pack_bf16x2(a, b);
           }
           tmem_st16(st + c * 16, w);
           if ((c + 1) % (4 / kParts) == 0) {
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(bar(P_FULL + t * kParts + c / (4 / kParts)));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(P_FULL + t * kParts + c / (4 / kParts)));   // one per warp: arrivals queue up
           }
         }
         float a, b;
@@ -698,7 +770,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       const int tok_end = min(it.tok0 + (t + 1) * TP, it.len);
       v_ring += 2 * N;
       if (n > 0 && ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(O_FULL + t), (step - 1) & 1, 0x319));
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(O_FULL + t), (step - 1) & 1, 0x319));
         if (!ok) break;
         tc_fence_after();
         const bool live = r < TP * G && tok < tok_end;

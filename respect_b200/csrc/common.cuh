@@ -99,6 +99,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int cod
   }
 }
 
+// The same for waits on a kernel's critical path: a read of %globaltimer takes several hundred
+// cycles, so the clock is looked at only after many tries.
+__device__ __forceinline__ bool mbar_wait_spin(uint32_t bar, uint32_t parity, int code) {
+#pragma unroll 1
+  for (uint32_t it = 0; it < 4096; ++it)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, code);
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
