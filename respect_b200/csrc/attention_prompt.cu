@@ -330,15 +330,26 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
 //
 // Warps 0-3 / 4-7: softmax of tile A / B, one row a thread (no exchange between
 // threads); warp 8: TMA (Q of the block, a ring of K and V tiles); warp 9: issues the
-// MMAs. The block is persistent: K / V and Q of its next work item arrive, and S of it
-// is computed, while the results of the last one are written out.
+// MMAs; warp 10: says which tiles are next. The block is persistent: K / V and Q of its
+// next work item arrive, and S of it is computed, while the results of the last one are
+// written out.
+//
+// Bound: the chain S -> softmax -> P V -> next S of a tile (S and P share tensor memory).
+// A step of 128 keys takes about 3,100 cycles, of which the two tiles' four products need
+// 2,048: 1,880 of softmax (1,024 of them the exponentials of a thread's 128 scores), 770 of
+// MMA that the other tile's softmax covers, the rest hand-overs. Measured: 32,768 tokens,
+// 32 / 8 heads 7.5 ms (1,170 TFLOP/s; a matrix product of the library holds 1,390 for that
+// long); 16 prompts of about 4,096, 28 / 4 heads 2.0 ms (950). Two threads a row
+// (16 softmax warps) measured slower (1,020), as did more of the exponentials on the FMA
+// pipe (a half: 1,050) and P in four parts (1,090).
 namespace tcp {
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kHalf = 128 * 64 * 2;              // 64 dims of 128 rows: 16 KB, 128-byte swizzle
 constexpr int kTile = 2 * kHalf;
-constexpr int kRing = 5;                         // K / V buffers
+constexpr int kRing = 4;                         // K / V buffers
 constexpr int kKVOff = 2 * kTile;                // after Q_A, Q_B
-constexpr int kBarOff = kKVOff + kRing * kTile;
+constexpr int kStageOff = kKVOff + kRing * kTile;  // results on their way out: 32 rows of 64 dims a softmax warp
+constexpr int kBarOff = kStageOff + 8 * 4096;
 constexpr int kItemOff = kBarOff + 256;          // announced items, 32 bytes each
 constexpr int kSmem = 1024 + kItemOff + 64;
 static_assert(kSmem <= 232448, "shared memory budget");
@@ -347,7 +358,7 @@ constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last war
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "register split");
 constexpr int kProducerWarp = 8, kMmaWarp = 9, kItemWarp = 10;
-constexpr int kParts = 2;                        // P is handed over in parts of 64 keys
+constexpr int kParts = 2;                        // P is handed over in parts of 128 / kParts keys
 constexpr int kItems = 2;                        // work items announced ahead
 enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + kRing, S_FULL = KV_EMPTY + kRing, P_FULL = S_FULL + 2,
        O_FULL = P_FULL + 2 * kParts, ITEM_FULL = O_FULL + 2, ITEM_EMPTY = ITEM_FULL + kItems, NBAR = ITEM_EMPTY + kItems };
@@ -378,6 +389,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_if(uint32_t bar, bool go) {   // without a branch
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+               "r"(static_cast<uint32_t>(go))
+               : "memory");
 }
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -466,6 +487,8 @@ __device__ __forceinline__ void item_of(const Dev& p, int unit, Item* it) {
 }
 }  // namespace tcp
 
+// kFlip: a negative scale, with which the largest weight is at the smallest S.
+template <bool kFlip>
 __global__ void __launch_bounds__(tcp::kThreads, 1)
     prompt_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
               const __grid_constant__ CUtensorMap tv, const Dev p) {
@@ -655,8 +678,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     const int r = q4 * 32 + lane;                      // row of the tile
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const uint32_t st = lane_base + kSCol + t * 128, ot = lane_base + kOCol + t * 128;
-    const bool flip = p.scale2 < 0.f;                  // the largest weight is then at the smallest S
-    const float masked = flip ? INFINITY : -INFINITY;
+    const float masked = kFlip ? INFINITY : -INFINITY;
     const uint64_t scale_pair = pair(p.scale2, p.scale2);
     uint32_t step = 0;                                 // S tiles consumed so far
     uint32_t v_ring = 0;                               // ring number of the item's V_0, less one
@@ -680,7 +702,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             if (c > last) s[c] = __float_as_uint(masked);
         }
         float top;
-        if (!flip) {
+        if (!kFlip) {
           float a = __uint_as_float(s[0]), b = __uint_as_float(s[1]), c = __uint_as_float(s[2]), d = __uint_as_float(s[3]);
 #pragma unroll
           for (int x = 4; x < 124; x += 8) {
@@ -706,7 +728,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(O_FULL + t), (step - 1) & 1, 0x317));
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 8; ++c) {
             uint32_t o[16];
             tmem_ld16_nowait(ot + c * 16, o);
@@ -732,35 +754,42 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             }
           }
           fence_proxy_async_smem();
+          __syncwarp();
         }
+        // One straight run of code, so that the exponentials (8 cycles each on their pipe) of one
+        // group of 16 overlap the sums, conversions and stores of the group before.
         const uint64_t neg_pair = pair(neg, neg);
-        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+        uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)}, y[2][8];
+        uint32_t w[2][8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
+        for (int c = 0; c <= 8; ++c) {
+          if (c < 8) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint64_t x = fma2(pair(__uint_as_float(s[c * 32 + 2 * e]), __uint_as_float(s[c * 32 + 2 * e + 1])), scale_pair, neg_pair);
-            float a, b;
-            uint64_t y;
-            if (e % 4 == 3) {   // a quarter on the FMA pipe: 2^x on the other one is the longer queue
-              y = exp2_pair(x);
-              unpair(y, a, b);
-            } else {
-              unpair(x, a, b);
-              a = fast_exp2(a);
-              b = fast_exp2(b);
-              y = pair(a, b);
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t x = fma2(pair(__uint_as_float(s[c * 16 + 2 * e]), __uint_as_float(s[c * 16 + 2 * e + 1])), scale_pair, neg_pair);
+              if (e == 7) {   // one pair of eight on the FMA pipe: the exponential's own is the longer queue
+                y[c & 1][e] = exp2_pair(x);
+              } else {
+                float a, b;
+                unpair(x, a, b);
+                y[c & 1][e] = pair(fast_exp2(a), fast_exp2(b));
+              }
             }
-            sum[e & 1] = add2(sum[e & 1], y);
-            w[e] = pack_bf16x2(a, b);
           }
-          tmem_st16(st + c * 16, w);
-          if ((c + 1) % (4 / kParts) == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(P_FULL + t * kParts + c / (4 / kParts)));   // one per warp: arrivals queue up
+          if (c > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float a, b;
+              unpair(y[(c - 1) & 1][e], a, b);
+              sum[e & 1] = add2(sum[e & 1], y[(c - 1) & 1][e]);
+              w[(c - 1) & 1][e] = pack_bf16x2(a, b);
+            }
+            tmem_st8(st + (c - 1) * 8, w[(c - 1) & 1]);
+            if (c % (8 / kParts) == 0) {
+              tmem_wait_st();     // the warp's own stores, all lanes
+              tc_fence_before();
+              mbar_arrive_if(bar(P_FULL + t * kParts + (c - 1) / (8 / kParts)), lane == 0);   // one per warp: arrivals queue up
+            }
           }
         }
         float a, b;
@@ -773,27 +802,41 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(O_FULL + t), (step - 1) & 1, 0x319));
         if (!ok) break;
         tc_fence_after();
+        // Rows lie apart in memory (256 bytes each): a warp's 64 dims of 32 rows pass through
+        // shared memory (16-byte pieces swizzled by row), so that a store covers 4 lines, not 32.
         const bool live = r < TP * G && tok < tok_end;
-        const int h = it.kvh * G + r % G;
-        uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(it.s0 + tok) * p.sot + h * p.soh;
+        const int64_t at = live ? static_cast<int64_t>(it.s0 + tok) * p.sot + (it.kvh * G + r % G) * p.soh : -1;
         const float inv = 1.f / l;
+        uint8_t* stage = smem + kStageOff + warp * 4096;
         bool nan = false;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(ot + c * 32, o);
-          tmem_wait_ld();
+          for (int c = 0; c < 2; ++c) {
+            uint32_t o[32];
+            tmem_ld32(ot + half * 64 + c * 32, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float a = __uint_as_float(o[e * 8 + 2 * x]) * inv, b = __uint_as_float(o[e * 8 + 2 * x + 1]) * inv;
-              nan |= a != a || b != b;
-              w[x] = pack_bf16x2(a, b);
+              for (int x = 0; x < 4; ++x) {
+                const float a = __uint_as_float(o[e * 8 + 2 * x]) * inv, b = __uint_as_float(o[e * 8 + 2 * x + 1]) * inv;
+                nan |= a != a || b != b;
+                w[x] = pack_bf16x2(a, b);
+              }
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((c * 4 + e) ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (live) *reinterpret_cast<uint4*>(out + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int row = x * 4 + (lane >> 3), piece = lane & 7;
+            const int64_t to = __shfl_sync(0xffffffffu, at, row);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((piece ^ (row & 7)) * 16));
+            if (to >= 0) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to + half * 64 + piece * 8) = v;
+          }
+          __syncwarp();
         }
         tc_fence_before();   // O read before the next item's P (and so its P V) is announced
         for (unsigned again = __ballot_sync(0xffffffffu, nan && live); again; again &= again - 1) {
@@ -851,10 +894,11 @@ int prompt_launch(const rb_prompt_args* a, cudaStream_t st) {
     if (r == RB_OK) r = encode_heads_3d(&tk, a->k, a->T, a->HK, skt, skh);
     if (r == RB_OK) r = encode_heads_3d(&tv, a->v, a->T, a->HK, svt, svh);
     if (r != RB_OK) return r;
-    if (cudaFuncSetAttribute(prompt_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, tcp::kSmem) != cudaSuccess)
+    const auto kern = p.scale2 < 0.f ? prompt_tc<true> : prompt_tc<false>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, tcp::kSmem) != cudaSuccess)
       return RB_ERR_CUDA;
     const int64_t grid = units < device_sm_count() ? units : device_sm_count();
-    return launch_k(prompt_tc, dim3(static_cast<unsigned>(grid)), dim3(tcp::kThreads), tcp::kSmem, st, true, tq, tk, tv, p);
+    return launch_k(kern, dim3(static_cast<unsigned>(grid)), dim3(tcp::kThreads), tcp::kSmem, st, true, tq, tk, tv, p);
   }
   const int TP = f32::kRows / G;
   const int64_t grid = (static_cast<int64_t>(a->T) / TP + a->B + 1) * a->HK;   // tiles at most
