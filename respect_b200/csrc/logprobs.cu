@@ -4,11 +4,16 @@
 //   m = max x, S = sum e^(x-m), T = sum (x-m) e^(x-m)
 //   log p(t) = x_t - m - log S,   entropy = log S - T / S
 //
-// Bound: the logits are read once from HBM. A block takes kChunk consecutive
-// entries of a row into registers, so max, sums and the chunk's best entries come
-// from that one read; a second, small kernel joins a row's chunks in order. The
-// chunk grid depends on V alone and each thread owns fixed entries of it, so a row
+// Bound: the logits are read once from HBM. A block takes kChunk consecutive entries of
+// a row into registers, so maxima, sums and the chunk's best entries come from that one
+// read; a second, small kernel joins a row's parts in order. Each warp sums relative to
+// its own maximum (one redux), so without alternatives no thread waits for another warp;
+// an entry costs an exponential (16 a cycle and SM, 70% of the time the read takes for
+// bf16) and about six other instructions, two entries at a time where there are packed
+// forms. The grid depends on V alone and each thread owns fixed entries of it, so a row
 // gives the same bits alone or among others, whatever its alignment.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_util.h"
 
@@ -16,13 +21,18 @@ namespace rb {
 namespace lp {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kPer = 32;                     // entries per thread
-constexpr int kChunk = kThreads * kPer;      // 8192
+constexpr int kBytes = 128;                  // of a row per thread
+template <typename T>
+struct Shape {
+  static constexpr int kPer = kBytes / sizeof(T);   // entries per thread: 32 fp32, 64 bf16
+  static constexpr int kChunk = kThreads * kPer;
+  static constexpr int W = 16 / sizeof(T);          // entries of a 16-byte piece
+};
 constexpr int kMaxTop = RB_LOGPROBS_MAX_TOP;
 constexpr float kLog2E = 1.4426950408889634f;
 
-// One chunk: max, S, T and whether a NaN was seen, then the best `top` keys.
-struct Stat { float m, s, t; int nan; };
+// One warp's entries: maximum (a NaN if there is one), S, T.
+struct Stat { float m, s, t, pad; };
 
 // Order of the alternatives as one integer: larger value first (NaN above all,
 // -0 equal to 0), then lower index. 0 is below every key.
@@ -41,163 +51,281 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t min64(uint64_t a, uint64_t b) { return a < b ? a : b; }
-// 32 keys, one per lane, descending by lane (bitonic network).
-__device__ __forceinline__ uint64_t warp_sort_desc(uint64_t k) {
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return max64(a, b); }
+__device__ __forceinline__ uint64_t smaller(uint64_t a, uint64_t b) { return min64(a, b); }
+// 32 values, one per lane, descending by lane (bitonic network).
+template <typename K>
+__device__ __forceinline__ K warp_sort_desc(K k) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int d = size >> 1; d > 0; d >>= 1) {
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, k, d);
+      const K o = __shfl_xor_sync(0xffffffffu, k, d);
       const bool up = (lane & size) != 0 && size < 32, low = (lane & d) == 0;
-      k = (low != up) ? max64(k, o) : min64(k, o);
+      k = (low != up) ? larger(k, o) : smaller(k, o);
     }
   return k;
 }
 // The 32 largest of two descending lists, descending.
-__device__ __forceinline__ uint64_t warp_merge_desc(uint64_t a, uint64_t b) {
+template <typename K>
+__device__ __forceinline__ K warp_merge_desc(K a, K b) {
   const int lane = threadIdx.x & 31;
-  uint64_t k = max64(a, __shfl_sync(0xffffffffu, b, 31 - lane));   // a bitonic list
+  K k = larger(a, __shfl_sync(0xffffffffu, b, 31 - lane));   // a bitonic list
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, k, d);
-    k = (lane & d) == 0 ? max64(k, o) : min64(k, o);
+    const K o = __shfl_xor_sync(0xffffffffu, k, d);
+    k = (lane & d) == 0 ? larger(k, o) : smaller(k, o);
   }
   return k;
 }
 
 // 2^((x - m) log2 e): the difference first, so that a large m costs no accuracy
 __device__ __forceinline__ float exp_diff(float d) { return fast_exp2(d * kLog2E); }
-
-// Sum over the block in a fixed order; every thread gets it.
-__device__ __forceinline__ float block_sum(float v, float* buf) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) s += buf[w];
-  return s;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float warp_max_nan(float a) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(a));
+  return r;
 }
 
-// Thread t owns entries base + (j * kThreads + t) * W + e, e < W, j < kPer / W (W
-// entries are 16 bytes): one 16-byte load where the row allows it.
+// A thread's entries stay as they were read (bf16 packed) and are widened at each use.
+// Thread t owns entries base + (j * kThreads + t) * W + e, e < W, j < 8: one 16-byte load
+// per j where the row allows it. Entries past the row and excluded ones are -inf.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int base, int V, int off, int size, float (&x)[kPer]) {
-  constexpr int W = 16 / sizeof(T);
-  const bool vec = (reinterpret_cast<uintptr_t>(row + base) & 15u) == 0;
+struct Entries {
+  uint32_t raw[kBytes / 4];
+  __device__ __forceinline__ float operator[](int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(raw[i]);
+    return __uint_as_float((i & 1) ? (raw[i / 2] & 0xFFFF0000u) : (raw[i / 2] << 16));
+  }
+  __device__ __forceinline__ void clear(int i) {   // entry i: -inf
+    if (sizeof(T) == 4) raw[i] = 0xFF800000u;
+    else raw[i / 2] = (i & 1) ? ((raw[i / 2] & 0xFFFFu) | 0xFF800000u) : ((raw[i / 2] & 0xFFFF0000u) | 0xFF80u);
+  }
+  __device__ __forceinline__ static int at(int i) {   // entry i: offset in the chunk
+    constexpr int W = Shape<T>::W;
+    return ((i / W) * kThreads + static_cast<int>(threadIdx.x)) * W + i % W;
+  }
+  __device__ __forceinline__ float max() const {      // a NaN if there is one
+    if (sizeof(T) == 4) {
+      float m = __uint_as_float(raw[0]);
 #pragma unroll
-  for (int j = 0; j < kPer / W; ++j) {
-    const int i0 = base + (j * kThreads + static_cast<int>(threadIdx.x)) * W;
-    if (vec && i0 + W <= V) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(row + i0));
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+      for (int i = 1; i < kBytes / 4; ++i) m = max_nan(m, __uint_as_float(raw[i]));
+      return m;
+    }
+    uint32_t m = raw[0];
 #pragma unroll
-      for (int e = 0; e < W; ++e)
-        x[j * W + e] = sizeof(T) == 4 ? __uint_as_float(u[e * sizeof(T) / 4])
-                                      : __uint_as_float((e & 1) ? (u[e / 2] & 0xFFFF0000u) : (u[e / 2] << 16));
+    for (int i = 1; i < kBytes / 4; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(raw[i]));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+  }
+  __device__ __forceinline__ void load(const T* row, int base, int V, int off, int size) {
+    constexpr int W = Shape<T>::W;
+    const bool vec = (reinterpret_cast<uintptr_t>(row + base) & 15u) == 0;
+    if (vec && base + Shape<T>::kChunk <= V) {
+#pragma unroll
+      for (int j = 0; j < kBytes / 16; ++j) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(row + base) + j * kThreads + threadIdx.x);
+        raw[4 * j] = v.x;
+        raw[4 * j + 1] = v.y;
+        raw[4 * j + 2] = v.z;
+        raw[4 * j + 3] = v.w;
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        if (i0 + e >= V) x[j * W + e] = -INFINITY;
-        else if (sizeof(T) == 4) x[j * W + e] = reinterpret_cast<const float*>(row)[i0 + e];
-        else x[j * W + e] = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[i0 + e]);
+      for (int j = 0; j < kBytes / 16; ++j) {
+        const int i0 = base + at(j * W);
+        if (vec && i0 + W <= V) {
+          const uint4 v = __ldcs(reinterpret_cast<const uint4*>(row + i0));
+          raw[4 * j] = v.x;
+          raw[4 * j + 1] = v.y;
+          raw[4 * j + 2] = v.z;
+          raw[4 * j + 3] = v.w;
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (sizeof(T) == 4) {
+              raw[4 * j + w] = i0 + w < V ? reinterpret_cast<const uint32_t*>(row)[i0 + w] : 0xFF800000u;
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+              const uint32_t lo = i0 + 2 * w < V ? h[i0 + 2 * w] : 0xFF80u, hi = i0 + 2 * w + 1 < V ? h[i0 + 2 * w + 1] : 0xFF80u;
+              raw[4 * j + w] = lo | (hi << 16);
+            }
+          }
+        }
       }
     }
-    if (i0 < off + size && i0 + W > off) {
+    if (base < off + size && base + Shape<T>::kChunk > off) {
 #pragma unroll
-      for (int e = 0; e < W; ++e)
-        if (i0 + e >= off && i0 + e - off < size) x[j * W + e] = -INFINITY;
+      for (int i = 0; i < Shape<T>::kPer; ++i) {
+        const int x = base + at(i);
+        if (x >= off && x - off < size) clear(i);
+      }
     }
   }
-}
+};
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads)
-    chunk_kernel(const T* __restrict__ logits, int64_t ld, int V, int off, int size, int top, int chunks,
-                 Stat* __restrict__ stats, uint64_t* __restrict__ best) {
-  constexpr int W = 16 / sizeof(T);
-  __shared__ float buf[kWarps];
-  __shared__ uint64_t lists[kWarps][32];
-  __shared__ uint64_t limit;
-  __shared__ int found;
-  __shared__ uint64_t cand[TOP ? kMaxTop * kPer : 1];
-  pdl_wait();
-  pdl_trigger();
-  const int chunk = blockIdx.x % chunks, row = blockIdx.x / chunks;
+// The chunk's best entries. A limit that at least `top` entries reach and few others do:
+// the top-th largest of 32 maxima, one per lane number. Entries from the limit up go to
+// shared memory in any order (their keys differ) and are ranked by counting. Where many
+// tie at the limit, the lowest indices among them are taken, in order; where too many
+// lie above it, or a NaN is among them, the best entry is taken `top` times.
+constexpr int kCand = 1024;
+struct TopShared {
+  float maxima[kWarps][32];
+  float limit;
+  int found, warp_count[kWarps];
+  uint64_t cand[kCand], round;
+};
+template <typename T>
+__device__ void choose(const Entries<T>& x, float mine, bool nan, int base, int V, int top, TopShared& sh, uint64_t* out) {
+  constexpr int kPer = Shape<T>::kPer, W = Shape<T>::W;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float x[kPer];
-  load_chunk(logits + row * ld, chunk * kChunk, V, off, size, x);
-
-  float m = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    m = fmaxf(m, x[i]);
-    nan |= x[i] != x[i];
-  }
-  uint64_t mine = 0;
-  if (TOP) {   // the thread's best key
+  const float limit = sh.limit;
+  // at -inf there are always too many
+  const bool crowded = limit == -INFINITY;
+  if (mine >= limit && !crowded && !nan) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = chunk * kChunk + ((i / W) * kThreads + static_cast<int>(threadIdx.x)) * W + i % W;
-      if (at < V) mine = max64(mine, key_of(x[i], at));
+      const float v = x[i];
+      if (v >= limit && base + x.at(i) < V) {
+        const int c = atomicAdd(&sh.found, 1);
+        if (c < kCand) sh.cand[c] = key_of(v, base + x.at(i));
+      }
     }
-    if (threadIdx.x == 0) found = 0;
-    lists[warp][lane] = warp_sort_desc(mine);
   }
-  m = warp_max(m);
-  if (lane == 0) buf[warp] = m;
-  nan = __syncthreads_or(nan);
-  m = buf[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, buf[w]);
-  if (TOP && warp == 0) {
-    // The top-th best of the threads' best keys: at least `top` entries reach it,
-    // and only the threads whose own best does can hold one of them.
-    uint64_t k = lists[0][lane];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) k = warp_merge_desc(k, lists[w][lane]);
-    if (lane == top - 1) limit = k;
-  }
-  const float ref = (m == -INFINITY || m == INFINITY) ? 0.f : m;
-  float s = 0.f, t = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float d = x[i] - ref, e = exp_diff(d);
-    s += e;
-    t += e > 0.f ? d * e : 0.f;   // an excluded or vanishing entry adds nothing
-  }
-  s = block_sum(s, buf);
-  t = block_sum(t, buf);
-  if (threadIdx.x == 0) stats[blockIdx.x] = Stat{m, s, t, nan};
-  if (TOP) {
-    const uint64_t lim = limit;   // written before block_sum's barriers
-    if (mine >= lim && mine != 0) {
+  __syncthreads();
+  int n = sh.found;
+  if (n > kCand || crowded || nan) {   // the same in every thread, as is every branch below
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = 0;
+    __syncthreads();
+    if (mine > limit && !nan) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int at = chunk * kChunk + ((i / W) * kThreads + static_cast<int>(threadIdx.x)) * W + i % W;
-        const uint64_t k = at < V ? key_of(x[i], at) : 0;
-        if (k != 0 && k >= lim) cand[atomicAdd(&found, 1)] = k;   // at most top threads come here
+        const float v = x[i];
+        if (v > limit && base + x.at(i) < V) {
+          const int c = atomicAdd(&sh.found, 1);
+          if (c < kCand) sh.cand[c] = key_of(v, base + x.at(i));
+        }
       }
     }
     __syncthreads();
-    const int n = found;
-    uint64_t* out = best + static_cast<int64_t>(blockIdx.x) * top;
-    for (int i = threadIdx.x; i < n; i += kThreads) {   // the order of cand[] does not matter: keys differ
-      const uint64_t k = cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand[j] > k;
-      if (rank < top) out[rank] = k;
+    n = sh.found;
+    if (nan || n > kCand - kMaxTop) {
+      uint64_t last = ~0ull;
+      for (int r = 0; r < top; ++r) {
+        if (threadIdx.x == 0) sh.round = 0;
+        __syncthreads();
+        uint64_t k = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const uint64_t c = base + x.at(i) < V ? key_of(x[i], base + x.at(i)) : 0;
+          if (c < last) k = max64(k, c);
+        }
+        atomicMax(reinterpret_cast<unsigned long long*>(&sh.round), static_cast<unsigned long long>(k));
+        __syncthreads();
+        last = sh.round;
+        if (threadIdx.x == 0) out[r] = last;
+        __syncthreads();
+      }
+      return;
     }
-    for (int i = n + static_cast<int>(threadIdx.x); i < top; i += kThreads) out[i] = 0;   // a chunk shorter than top
+    int ties = 0;         // taken so far, in index order: j, then thread, then entry
+#pragma unroll
+    for (int j = 0; j < kBytes / 16; ++j) {
+      if (ties < top) {
+        int here = 0;
+#pragma unroll
+        for (int e = 0; e < W; ++e) here += x[j * W + e] == limit && base + x.at(j * W + e) < V;
+        int sum = here;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        if (lane == 31) sh.warp_count[warp] = sum;
+        __syncthreads();
+        int at = ties + sum - here, all = 0;
+        for (int w = 0; w < kWarps; ++w) {
+          if (w < warp) at += sh.warp_count[w];
+          all += sh.warp_count[w];
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const int pos = base + x.at(j * W + e);
+          if (x[j * W + e] == limit && pos < V && at < top) sh.cand[n + at++] = key_of(limit, pos);
+        }
+        ties += all;
+        __syncthreads();
+      }
+    }
+    n += min(ties, top);
+  }
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t k = sh.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.cand[j] > k;
+    if (rank < top) out[rank] = k;
+  }
+  for (int i = n + static_cast<int>(threadIdx.x); i < top; i += kThreads) out[i] = 0;   // a chunk shorter than top
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads, TOP ? 3 : 4)
+    chunk_kernel(const T* __restrict__ logits, int64_t ld, int V, int off, int size, int top, int chunks,
+                 Stat* __restrict__ stats, uint64_t* __restrict__ best) {
+  __shared__ typename std::conditional<TOP, TopShared, int>::type shared;
+  pdl_wait();
+  pdl_trigger();
+  const int chunk = blockIdx.x % chunks, row = blockIdx.x / chunks;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, base = chunk * Shape<T>::kChunk;
+  Entries<T> x;
+  x.load(logits + row * ld, base, V, off, size);
+  const float mine = x.max();
+  const float m = warp_max_nan(mine);
+  if constexpr (TOP) {
+    if (threadIdx.x == 0) shared.found = 0;
+    shared.maxima[warp][lane] = mine;
+    __syncthreads();
+    if (warp == 0) {
+      float k = mine;
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) k = fmaxf(k, shared.maxima[w][lane]);
+      k = warp_sort_desc(k);
+      if (lane == top - 1) shared.limit = k;
+    }
+  }
+  // relative to the warp's maximum; an entry of -inf weighs nothing (a finite number times 0)
+  const float ref = (m == -INFINITY || m == INFINITY) ? 0.f : m;
+  float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < Shape<T>::kPer; i += 2) {
+    const float d0 = fmaxf(x[i] - ref, -1e30f), d1 = fmaxf(x[i + 1] - ref, -1e30f);
+    const float e0 = exp_diff(d0), e1 = exp_diff(d1);
+    s0 += e0;
+    s1 += e1;
+    t0 = fmaf(d0, e0, t0);
+    t1 = fmaf(d1, e1, t1);
+  }
+  const float s = warp_sum(s0 + s1), t = warp_sum(t0 + t1);
+  if (lane == 0) *reinterpret_cast<float4*>(stats + static_cast<int64_t>(blockIdx.x) * kWarps + warp) = make_float4(m, s, t, 0.f);
+  if constexpr (TOP) {
+    const bool nan = __syncthreads_or(mine != mine);
+    choose<T>(x, mine, nan, base, V, top, shared, best + static_cast<int64_t>(blockIdx.x) * top);
   }
 }
 
-// One warp per row: the chunks in order.
+// The row's sums in order, by one warp, and the chunks' best entries: a block per row with
+// alternatives (its warps share the lists), a warp per row without.
 constexpr int kJoinWarps = 4;
-template <typename T>
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     join_kernel(const T* __restrict__ logits, int64_t ld, int M, int V, const int64_t* __restrict__ tokens, int off,
                 int size, int top, int chunks, const Stat* __restrict__ stats, const uint64_t* __restrict__ best,
@@ -205,29 +333,41 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
                 int64_t* __restrict__ top_ids) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, row = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = TOP ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
   if (row >= M) return;
-  const Stat* st = stats + static_cast<int64_t>(row) * chunks;
-  float m = -INFINITY;
-  int nan = 0;
-  for (int c = lane; c < chunks; c += 32) {
-    m = fmaxf(m, st[c].m);
-    nan |= st[c].nan;
+  uint64_t k = 0;
+  if constexpr (TOP) {
+    __shared__ uint64_t lists[kJoinWarps][32];
+    const uint64_t* b = best + static_cast<int64_t>(row) * chunks * top;
+#pragma unroll 4
+    for (int c = warp; c < chunks; c += kJoinWarps) k = warp_merge_desc(k, lane < top ? b[static_cast<int64_t>(c) * top + lane] : uint64_t(0));
+    lists[warp][lane] = k;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) k = warp_merge_desc(k, lists[w][lane]);
   }
-  m = warp_max(m);
-  nan = __any_sync(0xffffffffu, nan);
-  float s = 0.f, t = 0.f;
-  for (int c = lane; c < chunks; c += 32) {
-    const Stat x = st[c];
-    if (x.m == -INFINITY) continue;
-    const float d = x.m - m, w = exp_diff(d);
-    s = fmaf(w, x.s, s);
-    t = fmaf(w, fmaf(d, x.s, x.t), t);
+  const int64_t parts = static_cast<int64_t>(chunks) * kWarps;
+  const float4* st = reinterpret_cast<const float4*>(stats + row * parts);
+  // running (m, s, t) per lane: one pass over the row's parts
+  float m = -INFINITY, s = 0.f, t = 0.f;
+#pragma unroll 4
+  for (int64_t c = lane; c < parts; c += 32) {
+    const float4 x = st[c];
+    const float hi = max_nan(m, x.x), ref = (hi == -INFINITY || hi == INFINITY) ? 0.f : hi;
+    // a side of -inf has nothing in it
+    const float da = fmaxf(m - ref, -1e30f), db = fmaxf(x.x - ref, -1e30f);
+    const float wa = exp_diff(da), wb = exp_diff(db);
+    t = wa * fmaf(da, s, t) + wb * fmaf(db, x.y, x.z);
+    s = wa * s + wb * x.y;
+    m = hi;
   }
-  s = warp_sum(s);
-  t = warp_sum(t);
+  const float top_m = warp_max_nan(m), ref = (top_m == -INFINITY || top_m == INFINITY) ? 0.f : top_m;
+  const float d = fmaxf(m - ref, -1e30f), w = exp_diff(d);
+  t = warp_sum(w * fmaf(d, s, t));
+  s = warp_sum(w * s);
   const float nan_f = __uint_as_float(0x7FC00000u);
-  const bool bad = nan || m == -INFINITY || m == INFINITY;
+  const bool bad = top_m != top_m || top_m == -INFINITY || top_m == INFINITY;
   const float logs = logf(s);
   if (lane == 0) {
     const int64_t tok = tokens[row];
@@ -238,55 +378,50 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
         if (sizeof(T) == 4) x = reinterpret_cast<const float*>(logits)[row * ld + tok];
         else x = bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(logits)[row * ld + tok]);
       }
-      v = x - m - logs;
+      v = x - top_m - logs;
     }
     logprob[row] = v;
     entropy[row] = bad ? nan_f : logs - t / s;
   }
-  if (top > 0) {
-    uint64_t k = 0;
-    for (int c = 0; c < chunks; ++c) {
-      const uint64_t* b = best + (static_cast<int64_t>(row) * chunks + c) * top;
-      k = warp_merge_desc(k, lane < top ? b[lane] : 0);
-    }
+  if constexpr (TOP) {
     if (lane < top) {
-      top_lp[static_cast<int64_t>(row) * top + lane] = bad ? nan_f : value_of(k) - m - logs;
+      top_lp[static_cast<int64_t>(row) * top + lane] = bad ? nan_f : value_of(k) - top_m - logs;
       top_ids[static_cast<int64_t>(row) * top + lane] = index_of(k);
     }
   }
 }
 
-__host__ inline int64_t chunks_of(int V) { return (static_cast<int64_t>(V) + kChunk - 1) / kChunk; }
+__host__ inline int64_t chunks_of(int V, int chunk) { return (static_cast<int64_t>(V) + chunk - 1) / chunk; }
 
 template <typename T>
 int run(const void* logits, int64_t ld, int M, int V, const int64_t* tokens, int off, int size, int top, float* logprob,
         float* entropy, float* top_lp, int64_t* top_ids, void* ws, cudaStream_t st) {
-  const int chunks = static_cast<int>(chunks_of(V));
+  const int chunks = static_cast<int>(chunks_of(V, Shape<T>::kChunk));
   const T* x = static_cast<const T*>(logits);
   Stat* stats = static_cast<Stat*>(ws);
-  uint64_t* best = reinterpret_cast<uint64_t*>(stats + static_cast<int64_t>(M) * chunks);
+  uint64_t* best = reinterpret_cast<uint64_t*>(stats + static_cast<int64_t>(M) * chunks * kWarps);
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(M) * chunks));
-  const int r = top > 0 ? launch_k(chunk_kernel<T, true>, grid, dim3(kThreads), 0, st, true, x, ld, V, off, size, top,
-                                   chunks, stats, best)
-                        : launch_k(chunk_kernel<T, false>, grid, dim3(kThreads), 0, st, true, x, ld, V, off, size, top,
-                                   chunks, stats, best);
-  if (r != RB_OK) return r;
-  return launch_k(join_kernel<T>, dim3((M + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, st, true, x, ld, M,
-                  V, tokens, off, size, top, chunks, stats, best, logprob, entropy, top_lp, top_ids);
+  auto go = [&](auto chunk, auto join, int rows_per_block) {
+    const int r = launch_k(chunk, grid, dim3(kThreads), 0, st, true, x, ld, V, off, size, top, chunks, stats, best);
+    if (r != RB_OK) return r;
+    return launch_k(join, dim3((M + rows_per_block - 1) / rows_per_block), dim3(32 * kJoinWarps), 0, st, true, x, ld, M, V, tokens,
+                    off, size, top, chunks, stats, best, logprob, entropy, top_lp, top_ids);
+  };
+  return top > 0 ? go(chunk_kernel<T, true>, join_kernel<T, true>, 1) : go(chunk_kernel<T, false>, join_kernel<T, false>, kJoinWarps);
 }
 
 }  // namespace lp
 
 size_t logprobs_workspace(int M, int V, int top) {
-  if (M <= 0 || V <= 0 || top < 0) return 0;
-  return static_cast<size_t>(M) * lp::chunks_of(V) * (sizeof(lp::Stat) + sizeof(uint64_t) * top);
+  if (M <= 0 || V <= 0 || top < 0) return 0;   // of fp32's chunks, the smaller ones
+  return static_cast<size_t>(M) * lp::chunks_of(V, lp::Shape<float>::kChunk) * (sizeof(lp::Stat) * lp::kWarps + sizeof(uint64_t) * top);
 }
 
 int logprobs_launch(const void* logits, int dtype, int64_t ld, int M, int V, const int64_t* tokens, int off, int size,
                     int top, float* logprob, float* entropy, float* top_lp, int64_t* top_ids, void* ws,
                     cudaStream_t st) {
-  if (static_cast<int64_t>(M) * lp::chunks_of(V) > INT32_MAX) return RB_ERR_CAPACITY;
-  if (V > INT32_MAX - lp::kChunk) return RB_ERR_CAPACITY;
+  if (static_cast<int64_t>(M) * lp::chunks_of(V, lp::Shape<float>::kChunk) > INT32_MAX) return RB_ERR_CAPACITY;
+  if (V > INT32_MAX - lp::Shape<uint16_t>::kChunk) return RB_ERR_CAPACITY;
   if (off > V) off = V;
   if (size > V - off) size = V - off;
   return dtype == RB_F32 ? lp::run<float>(logits, ld, M, V, tokens, off, size, top, logprob, entropy, top_lp, top_ids, ws, st)

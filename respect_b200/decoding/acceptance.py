@@ -8,6 +8,7 @@ tokens were under the same exclusion, with the entropy and the best alternatives
 """
 from __future__ import annotations
 
+import functools
 from typing import Callable, NamedTuple
 
 import torch
@@ -58,21 +59,30 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
     if offset < 0 or size < 0 or V == 0:
         raise ValueError("token_logprobs: bad excluded range or empty vocabulary")
     x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
-    x = x.reshape(-1, V)
+    lead = x.shape[:-1]
+    if x.dim() != 2:
+        x, tokens = x.reshape(-1, V), tokens.reshape(-1)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     M, dev = x.shape[0], x.device
-    tok = tokens.reshape(-1).contiguous()
-    lp, ent = torch.empty(2, M, dtype=torch.float32, device=dev).unbind(0)
-    tlp = torch.empty(M, top, dtype=torch.float32, device=dev) if top else None
-    ids = torch.empty(M, top, dtype=torch.int64, device=dev) if top else None
-    nbytes = _lib.lib().rb_token_logprobs_workspace(M, V, top)
+    out = torch.empty((2 + top) * M, dtype=torch.float32, device=dev)
+    ids = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
+    lp, ent = out[:M], out[M:2 * M]
+    tlp = out[2 * M:].view(*lead, top) if top else None
+    nbytes = _scratch_bytes(M, V, top)
     ws = _lib.scratch(x, nbytes)
     _lib.launch("rb_token_logprobs", x, x.data_ptr(), _lib.dtype_code(x.dtype), x.stride(0) if M > 1 else V, M, V,
-                tok.data_ptr(), min(int(offset), V), min(int(size), V), int(top), lp.data_ptr(), ent.data_ptr(),
+                tokens.data_ptr(), min(offset, V), min(size, V), top, lp.data_ptr(), ent.data_ptr(),
                 tlp.data_ptr() if top else None, ids.data_ptr() if top else None,
                 ws.data_ptr() if ws is not None else None, nbytes)
-    lead = tokens.shape
-    return TokenLogprobs(lp.reshape(lead), ent.reshape(lead), tlp.reshape(*lead, top) if top else None,
-                         ids.reshape(*lead, top) if top else None)
+    if len(lead) != 1:
+        lp, ent = lp.view(lead), ent.view(lead)
+    return TokenLogprobs(lp, ent, tlp, ids)
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(M: int, V: int, top: int) -> int:
+    return _lib.lib().rb_token_logprobs_workspace(M, V, top)
 
 
 def walk(tree: Trie, first: int, cap: int, eos: int,

@@ -107,7 +107,7 @@ class PagedKVCache:
             raise ValueError(f"{name} holds {x.numel()} entries, expected {n}")
         if x.numel() > _lib.PAGES_MAX_LIST:
             raise ValueError(f"{name}: at most {_lib.PAGES_MAX_LIST} sequences per call")
-        return x.contiguous()
+        return x if x.is_contiguous() else x.contiguous()
 
     def _call(self, name: str, *args) -> None:
         _lib.launch(name, self.store, self._ref, *args)

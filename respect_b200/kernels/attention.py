@@ -18,6 +18,7 @@ kernel: what a sequence gets does not depend on what else the call carries.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -77,26 +78,28 @@ def fused_attn_hyb(q, kp, vp, kn, vn, msk, sm_scale=None,
     return attn_call(q, kp, vp, kn, vn, msk, out, sm_scale)
 
 
-def _rows(t: torch.Tensor, name: str, dims: int, like: torch.Tensor) -> torch.Tensor:
-    """t with the layout the kernels read (unit inner stride, rows in whole 16-byte pieces); a copy only if it lacks it."""
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+def _laid_out(t: torch.Tensor) -> bool:
+    """Unit inner stride, everything else in whole 16-byte pieces."""
+    st = t.stride()
+    odd = 0
+    for x in st[:-1]:
+        odd |= x                     # a negative stride cannot occur; any low bit set shows
+    return st[-1] == 1 and odd % (16 // t.element_size()) == 0 and t.data_ptr() % 16 == 0
+
+
+def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    """t with the layout the kernels read; a copy only if it lacks it."""
     if t.dtype != like.dtype or t.device != like.device:
         raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    unit = 16 // t.element_size()
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % unit or s < 0 for s in st[:-1]):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t if _laid_out(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _out(out, q: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    unit = 16 // q.element_size()
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
-    if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % unit for s in out.stride()[:-1]):
+    if not _laid_out(out):
         raise ValueError("out needs a unit inner stride and rows in whole 16-byte pieces")
     return out
 
@@ -104,9 +107,7 @@ def _out(out, q: torch.Tensor) -> torch.Tensor:
 def _int32(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != dims:
         raise TypeError(f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        t = t.contiguous()
-    return t
+    return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
 
 
 def _check_heads(q: torch.Tensor, heads_kv: int, dim: int) -> None:
@@ -133,15 +134,23 @@ def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
     cu = _int32(cu_seqlens, "cu_seqlens", 1, q.device)
     if cu.numel() < 1:
         raise ValueError("cu_seqlens holds one entry more than there are sequences")
-    q, k, v = _rows(q, "q", 3, q), _rows(k, "k", 3, q), _rows(v, "v", 3, q)
+    q, k, v = _rows(q, "q", q), _rows(k, "k", q), _rows(v, "v", q)
     y = _out(out, q)
     T, H, D = q.shape
-    a = _lib.PromptArgs(_lib.dtype_code(q.dtype), cu.numel() - 1, T, H, k.shape[1], D,
-                        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                        v.data_ptr(), v.stride(0), v.stride(1), cu.data_ptr(), y.data_ptr(), y.stride(0), y.stride(1),
-                        float(D ** -0.5 if sm_scale is None else sm_scale), int(out is None))
-    _lib.launch("rb_prompt_attn", q, ctypes.byref(a))
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), y.stride()
+    a = _lib.pack_prompt_args(_lib.dtype_code(q.dtype), cu.numel() - 1, T, H, k.shape[1], D, q.data_ptr(), sq[0], sq[1],
+                              k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], cu.data_ptr(),
+                              y.data_ptr(), so[0], so[1], D ** -0.5 if sm_scale is None else sm_scale, out is None)
+    _lib.launch("rb_prompt_attn", q, a)
     return y
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_bytes(B: int, H: int, HK: int, page_size: int, width: int, max_length: int) -> int:
+    """Scratch of a paged call: a function of its sizes."""
+    a = _lib.PagedArgs(dtype=_lib.RB_BF16, B=B, H=H, HK=HK, D=128, page_size=page_size, width=width, ld_table=width,
+                       max_length=max_length, q=16, out=16, lengths=16, table=16)
+    return _lib.lib().rb_paged_attn_workspace(ctypes.byref(a))
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=None, ahead=0, max_length=None, out=None):
@@ -172,15 +181,17 @@ def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=Non
             raise ValueError(f"{seqs.numel()} seqs for {B} queries")
     if ahead < 0 or (max_length is not None and max_length < 1):
         raise ValueError("ahead must not be negative, max_length must be positive")
-    q, k, v = _rows(q, "q", 3, q), _rows(k_pages, "k_pages", 4, q), _rows(v_pages, "v_pages", 4, q)
+    q, k, v = _rows(q, "q", q), _rows(k_pages, "k_pages", q), _rows(v_pages, "v_pages", q)
     y = _out(out, q)
-    a = _lib.PagedArgs(_lib.dtype_code(q.dtype), B, H, k.shape[1], D, q.data_ptr(), q.stride(0), q.stride(1),
-                       k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                       v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k.shape[0], k.shape[2],
-                       table.data_ptr(), max(table.stride(0), width), width, rows, lengths.data_ptr(),
-                       seqs.data_ptr() if seqs is not None else None, int(ahead), int(max_length or 0),
-                       y.data_ptr(), y.stride(0), y.stride(1), float(D ** -0.5 if sm_scale is None else sm_scale))
-    nbytes = _lib.lib().rb_paged_attn_workspace(ctypes.byref(a))
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), y.stride()
+    pages, HK, page_size, _ = k.shape
+    bound = int(max_length or 0)
+    a = _lib.pack_paged_args(_lib.dtype_code(q.dtype), B, H, HK, D, q.data_ptr(), sq[0], sq[1],
+                             k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], pages, page_size,
+                             table.data_ptr(), max(table.stride(0), width), width, rows, lengths.data_ptr(),
+                             seqs.data_ptr() if seqs is not None else 0, ahead, bound, y.data_ptr(), so[0], so[1],
+                             D ** -0.5 if sm_scale is None else sm_scale)
+    nbytes = _paged_bytes(B, H, HK, page_size, width, bound)
     ws = _lib.scratch(q, nbytes)
-    _lib.launch("rb_paged_attn", q, ctypes.byref(a), ws.data_ptr() if ws is not None else None, nbytes)
+    _lib.launch("rb_paged_attn", q, a, ws.data_ptr() if ws is not None else None, nbytes)
     return y

@@ -176,3 +176,14 @@ def test_plain_page_model():
     assert "".join(m.tokens(1)) == "abcdefx24"
     m.truncate(1, 0)
     assert m.refs == [2, 1, 0, 1, 0, 0]
+
+
+def test_packed_arguments_have_the_layout_of_the_mirrors():
+    """The bytes the Python layer fills equal the ctypes mirrors of the C structures, field by field."""
+    prompt = list(range(1, 20)) + [0.5, 1]
+    paged = list(range(1, 30)) + [0.5]
+    for pack, mirror, values in ((_lib.pack_prompt_args, _lib.PromptArgs, prompt),
+                                 (_lib.pack_paged_args, _lib.PagedArgs, paged)):
+        packed = pack(*values)
+        want = bytes(mirror(*values))
+        assert want.startswith(packed) and not any(want[len(packed):])
