@@ -10,10 +10,11 @@
 // itself: it takes consecutive chunks (as many as the launch has too many of) in tiles of
 // 16 keys through its own ring of asynchronous copies, which runs on across chunks.
 //
-// bf16: S and P V on m16n8k16 tiles, 16 query heads of the group per tile; P enters
-// P V as two bf16 parts (hi + lo), so a weight is good to 2^-16 and the result is
-// rounded once, at the end. fp32: three tf32 products per term, each step from zero and
-// added in fp32.
+// bf16: S^T = K Q^T and O^T = V^T P^T on m16n8k16 tiles, so that the group's heads are the
+// 8 (or 16) columns: a group of up to 8 wastes no rows and needs half the accumulators. P
+// enters as two bf16 parts (hi + lo), so a weight is good to 2^-16 and the result is
+// rounded once, at the end. Where pages hold whole tiles, a tile is four TMA boxes. fp32:
+// three tf32 products per term, each step from zero and added in fp32.
 #include "common.cuh"
 #include "host_util.h"
 
@@ -21,18 +22,21 @@ namespace rb {
 namespace pg {
 
 constexpr int kD = 128;
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kThreads = 32;               // a block is one warp: they share nothing, and spread evenly
 constexpr int kKeys = 16;                  // keys of a tile
+#ifndef RULE
+#define RULE 2
+#endif
 constexpr int kStages = 3;
 constexpr int kRows = 16;                  // query heads of a block
-constexpr int kMinChunk = 64, kMaxChunk = 2048;
+constexpr int kMinChunk = 32, kMaxChunk = 2048;
 
 // Keys per chunk of a sequence of `len` tokens: 64 up to 4,096 tokens, then doubled each
 // time the length is four times larger. A chunk's result costs G x 520 bytes written and
 // read against 512 bytes a key (bf16): 6% of the traffic for a group of 4 at 64.
 __host__ __device__ inline int chunk_of(int len) {
   int c = kMinChunk;
-  while (c < kMaxChunk && static_cast<int64_t>(c) * c < len) c *= 2;
+  while (c < kMaxChunk && static_cast<int64_t>(RULE) * c * c < len) c *= 2;
   return c;
 }
 __host__ __device__ inline int chunks_of(int len) {
@@ -43,7 +47,7 @@ __host__ __device__ inline int chunks_of(int len) {
 __host__ inline int max_chunks(int len) {
   int n = 1;
   for (int c = kMinChunk; c <= kMaxChunk; c *= 2) {   // the longest length each size serves
-    const int64_t top = c < kMaxChunk ? static_cast<int64_t>(c) * c : len;
+    const int64_t top = c < kMaxChunk ? static_cast<int64_t>(RULE) * c * c : len;
     const int x = static_cast<int>(top < len ? top : len);
     const int k = chunks_of(x);
     n = k > n ? k : n;
@@ -110,7 +114,7 @@ __device__ __forceinline__ bool item_of(const Dev& p, Item* it) {
   it->table = p.table + row * p.ld_table;
   it->chunk = chunk_of(it->len);
   it->chunks = chunks_of(it->len);
-  it->c0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * p.per_warp;
+  it->c0 = blockIdx.x * p.per_warp;
   if (it->c0 >= it->chunks) return false;
   it->k0 = it->c0 * it->chunk;
   it->k1 = min(static_cast<int64_t>(it->len), it->k0 + static_cast<int64_t>(p.per_warp) * it->chunk);
@@ -250,8 +254,8 @@ __device__ __forceinline__ void finish(const Dev& p, const Item& it, float* part
 
 constexpr int kTile16 = 2 * kKeys * kD * 2, kTile32 = 2 * kKeys * kD * 4;
 constexpr int kQPitch = kD + 4;            // floats per staged fp32 query row: ldmatrix without bank conflicts
-constexpr int smem16() { return kWarps * kStages * kTile16; }
-constexpr int smem32() { return kWarps * kStages * kTile32 + 2 * kRows * kQPitch * 4; }
+constexpr int smem16() { return 1024 + kStages * kTile16 + 64; }   // ring, mbarriers
+constexpr int smem32() { return kStages * kTile32 + kRows * kQPitch * 4; }
 static_assert(smem32() <= 232448, "shared memory budget");
 
 // The running state of one warp's 16 rows, and what a tile does to it.
@@ -347,9 +351,37 @@ __device__ __forceinline__ void run_tiles(const Dev& p, const Item& it, uint32_t
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 2) paged_bf16(const Dev p, float* __restrict__ part) {
-  extern __shared__ __align__(128) uint8_t sm[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+// ---------------------------------------------------------------- bf16
+constexpr int kHalf16 = kKeys * 128;       // 64 dims of a tile's rows: 128 bytes each, 16-byte pieces swizzled by row & 7
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int slot, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 bf16 matrix, one register a lane
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// NT: columns of 8 query heads. kTma: pages hold whole tiles (page size % 16 == 0), so a tile
+// lies in one page; else its rows are gathered one by one.
+template <int NT, bool kTma>
+__global__ void __launch_bounds__(kThreads, 8)
+    paged_bf16(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Dev p,
+               float* __restrict__ part) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int lane = threadIdx.x, g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(sm), bars = ring + kStages * kTile16;
+  if (kTma && lane == 0) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + i * 8, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   pdl_wait();
   pdl_trigger();
   Item it;
@@ -357,49 +389,226 @@ __global__ void __launch_bounds__(kThreads, 2) paged_bf16(const Dev p, float* __
     if (it.len == 0) write_empty<uint16_t>(p, it);
     return;
   }
-  // queries as A fragments: rows g, g + 8 (heads past the group are zero)
-  uint32_t qa[kD / 16][4];
+  const int tiles = (it.k1 - it.k0 + kKeys - 1) / kKeys, per_chunk = it.chunk / kKeys;
+  // the page of tile t (kTma: of the tile; else of this lane's key), looked up one tile ahead
+  auto page_at = [&](int t) {
+    if (!kTma) return page_of(p, it, t);
+    if (t >= tiles) return -1;
+    const int x = it.table[(it.k0 + t * kKeys) / p.page_size];
+    return x < p.pages ? x : -1;
+  };
+  auto get = [&](int t, int page, int stage) -> uint32_t {   // starts tile t; which of its keys there are
+    const uint32_t dst = ring + stage * kTile16;
+    const int key = it.k0 + t * kKeys;
+    if (kTma) {
+      if (lane == 0) {
+        const uint32_t bar = bars + stage * 8;
+        if (page >= 0) {
+          const int slot = key % p.page_size;
+          mbar_arrive_expect_tx(bar, kTile16);
+          tma_box(dst, &tk, bar, 0, slot, it.kvh, page);
+          tma_box(dst + kHalf16, &tk, bar, 64, slot, it.kvh, page);
+          tma_box(dst + 2 * kHalf16, &tv, bar, 0, slot, it.kvh, page);
+          tma_box(dst + 3 * kHalf16, &tv, bar, 64, slot, it.kvh, page);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
+      const int n = it.k1 - key;
+      return page < 0 ? 0u : n < kKeys ? (1u << n) - 1u : 0xFFFFu;
+    }
+    const int slot = (key + (lane & 15)) % p.page_size, piece = lane & 15;
+    const int64_t ko = page < 0 ? 0 : page * p.skp + slot * p.sks, vo = page < 0 ? 0 : page * p.svp + slot * p.svs;
+    const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
+    const uint16_t* k = static_cast<const uint16_t*>(p.k) + it.kvh * p.skh + piece * 8;
+    const uint16_t* v = static_cast<const uint16_t*>(p.v) + it.kvh * p.svh + piece * 8;
+#pragma unroll
+    for (int i = 0; i < kKeys / 2; ++i) {
+      const int row = i * 2 + (lane >> 4);
+      const int64_t a = __shfl_sync(0xffffffffu, ko, row), b = __shfl_sync(0xffffffffu, vo, row);
+      const bool ok = valid >> row & 1;
+      const uint32_t at = dst + (piece >> 3) * kHalf16 + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
+      copy16(at, ok ? static_cast<const void*>(k + a) : p.q, ok ? 16u : 0u);   // a row that does not exist reads nothing
+      copy16(at + 2 * kHalf16, ok ? static_cast<const void*>(v + b) : p.q, ok ? 16u : 0u);
+    }
+    return valid;
+  };
+
+  uint32_t valid[kStages];
+  int page = page_at(0);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    valid[s] = s < tiles ? get(s, page, s) : 0;
+    page = page_at(s + 1);
+    if (!kTma) copy_commit();
+  }
+  // queries as B fragments: column g of each eight (heads past the group are zero)
+  uint32_t qb[NT][kD / 16][2];
   const uint16_t* q = static_cast<const uint16_t*>(p.q) + it.b * p.sqb + it.h0 * p.sqh;
 #pragma unroll
-  for (int kk = 0; kk < kD / 16; ++kk)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = g + (e & 1) * 8;
-      qa[kk][e] = r < it.nh ? *reinterpret_cast<const uint32_t*>(q + r * p.sqh + kk * 16 + (e >> 1) * 8 + c * 2) : 0u;
-    }
-  State st;
-  run_tiles<uint16_t>(p, it, smem_u32(sm) + warp * kStages * kTile16, part, st, [&](uint32_t K, uint32_t valid) {
-    const uint32_t V = K + kKeys * kD * 2;
-    // S: two 8-key tiles; ldmatrix matrices = (keys 0-7, 8-15) x (k halves)
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    const int kr = (lane & 7) + (lane >> 4) * 8;
+    for (int kk = 0; kk < kD / 16; ++kk)
 #pragma unroll
-    for (int kk = 0; kk < kD / 16; ++kk) {
-      uint32_t kb[4];
-      ldsm4(K + kr * (kD * 2) + (((kk * 2 + (lane >> 3 & 1)) ^ (kr & 7)) * 16), kb);
-      mma_bf16_16816(sc[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], kb[0], kb[1]);
-      mma_bf16_16816(sc[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], kb[2], kb[3]);
-    }
-    st.weigh(sc, valid, p.scale2);
-    // P as A fragments, in two parts
-    uint32_t hi[4], lo[4];
+      for (int e = 0; e < 2; ++e)
+        qb[n][kk][e] = n * 8 + g < it.nh ? *reinterpret_cast<const uint32_t*>(q + (n * 8 + g) * p.sqh + kk * 16 + e * 8 + c * 2) : 0u;
+  // O^T: rows = dims 16 d + g, + 8; columns = heads 8 n + 2 c, + 1, as are m and l (l: this lane's keys)
+  float o[kD / 16][NT][4], m[NT][2], l[NT][2];
+  auto reset = [&] {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = sc[e >> 1][(e & 1) * 2], b = sc[e >> 1][(e & 1) * 2 + 1];
-      hi[e] = pack_bf16x2(a, b);
-      lo[e] = pack_bf16x2(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xFFFF0000u));
-    }
-    const int vr = lane & 15;
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int n = 0; n < kD / 16; ++n) {
-      uint32_t vb[4];
-      ldsm4_t(V + vr * (kD * 2) + (((n * 2 + (lane >> 4)) ^ (vr & 7)) * 16), vb);
-      mma_bf16_16816(st.o[2 * n], hi[0], hi[1], hi[2], hi[3], vb[0], vb[1]);
-      mma_bf16_16816(st.o[2 * n], lo[0], lo[1], lo[2], lo[3], vb[0], vb[1]);
-      mma_bf16_16816(st.o[2 * n + 1], hi[0], hi[1], hi[2], hi[3], vb[2], vb[3]);
-      mma_bf16_16816(st.o[2 * n + 1], lo[0], lo[1], lo[2], lo[3], vb[2], vb[3]);
+      for (int d = 0; d < kD / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][n][e] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
     }
-  });
+  };
+  reset();
+  int left = per_chunk, chunk = it.c0;
+  uint32_t phase = 0;
+  for (int t0 = 0; t0 < tiles; t0 += kStages, phase ^= 1) {
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) {
+      const int t = t0 + s;
+      if (t >= tiles) break;
+      constexpr int kAhead = kStages - 1;
+      const int sn = (s + kAhead) % kStages;   // the stage read last
+      valid[sn] = t + kAhead < tiles ? get(t + kAhead, page, sn) : 0;
+      page = page_at(t + kAhead + 1);
+      const uint32_t K = ring + s * kTile16, V = K + 2 * kHalf16, live = valid[s];
+      if (kTma) {
+        if (!__all_sync(0xffffffffu, mbar_wait_spin(bars + s * 8, phase, 0x321))) {   // an error flag is up: see the copies out
+          for (int x = t; x < min(tiles, t + kStages); ++x) mbar_wait(bars + x % kStages * 8, x / kStages & 1, 0x321);
+          return;
+        }
+        if (live != 0xFFFFu && live != 0u) {
+          // slots past the last token hold whatever was there: zero weights would not silence it
+          const int n = __popc(live);
+          for (int x = lane; x < kKeys * 16; x += 32)
+            if ((x >> 4) >= n)
+              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(V + ((x >> 3) & 1) * kHalf16 + (x >> 4) * 128 + (x & 7) * 16), "r"(0) : "memory");
+        }
+      } else {
+        copy_commit();
+        copy_wait<kAhead>();
+      }
+      __syncwarp();
+      if (live) {   // the same in every lane
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+        const int kr = lane & 15;                                   // ldmatrix rows: keys 0-7, 8-15, then the next 8 dims
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          uint32_t a[4];
+          const int piece = kk * 2 + (lane >> 4);
+          ldsm4(K + (piece >> 3) * kHalf16 + kr * 128 + (((piece & 7) ^ (kr & 7)) * 16), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_bf16_16816(sc[n], a[0], a[1], a[2], a[3], qb[n][kk][0], qb[n][kk][1]);
+        }
+        uint32_t hi[NT][2], lo[NT][2];
+        float alpha[NT][2];
+        bool same = true;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {   // column 2 c + e: this lane has keys g and g + 8
+            float& x = sc[n][e];
+            float& y = sc[n][2 + e];
+            x = (live >> g & 1) ? x * p.scale2 : -INFINITY;
+            y = (live >> (g + 8) & 1) ? y * p.scale2 : -INFINITY;
+            float mx = fmaxf(x, y);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx = fmaxf(mx, m[n][e]);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            alpha[n][e] = fast_exp2(m[n][e] - ref);
+            same &= alpha[n][e] == 1.f;
+            m[n][e] = mx;
+            x = fast_exp2(x - ref);
+            y = fast_exp2(y - ref);
+            l[n][e] = fmaf(l[n][e], alpha[n][e], x + y);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {   // keys g, then g + 8: rows of an 8 x 8 matrix, turned into columns
+            const float x = sc[n][2 * h], y = sc[n][2 * h + 1];
+            const uint32_t u = pack_bf16x2(x, y);
+            hi[n][h] = transpose8(u);
+            lo[n][h] = transpose8(pack_bf16x2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
+          }
+        }
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+          for (int d = 0; d < kD / 16; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][n][e] *= alpha[n][e & 1];
+        }
+        const int vr = (lane & 7) + (lane >> 4) * 8;                // ldmatrix rows: keys 0-7 (dims 0-7, 8-15), keys 8-15
+#pragma unroll
+        for (int d = 0; d < kD / 16; ++d) {
+          uint32_t a[4];
+          const int piece = d * 2 + (lane >> 3 & 1);
+          ldsm4_t(V + (piece >> 3) * kHalf16 + vr * 128 + (((piece & 7) ^ (vr & 7)) * 16), a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
+            mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+          }
+        }
+        __syncwarp();                      // the stage has been read before it is filled again
+      }
+      if (--left == 0 || t + 1 == tiles) { // the chunk is done
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float sum = l[n][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int r = n * 8 + c * 2 + e;
+            bool nan = false;
+            if (r < it.nh) {
+              if (it.chunks == 1) {
+                const bool some = sum > 0.f || sum != sum;   // no token at all: zeros
+                uint16_t* dst = out_at<uint16_t>(p, it, r) + g;
+#pragma unroll
+                for (int d = 0; d < kD / 16; ++d)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const float y = some ? o[d][n][h * 2 + e] / sum : 0.f;
+                    nan |= y != y;
+                    dst[d * 16 + h * 8] = f32_to_bf16_bits(y);
+                  }
+              } else {
+                float* dst = acc_at(p, part, it, r, chunk) + g;
+#pragma unroll
+                for (int d = 0; d < kD / 16; ++d)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    nan |= o[d][n][h * 2 + e] != o[d][n][h * 2 + e];
+                    dst[d * 16 + h * 8] = o[d][n][h * 2 + e];
+                  }
+                if (g == 0) *ml_at(p, part, it, r, chunk) = make_float2(m[n][e], sum);
+              }
+            }
+            const unsigned again = __ballot_sync(0xffffffffu, nan);
+            if (again) {
+              for (int x = 0; x < 4; ++x)
+                if (again & (0x11111111u << x)) redo_row<uint16_t>(p, it, part, n * 8 + x * 2 + e, chunk);
+            }
+          }
+        reset();
+        left = per_chunk;
+        ++chunk;
+      }
+    }
+  }
 }
 
 // fp32. ldmatrix moves 8 x 4 fp32 blocks as it moves 8 x 8 bf16 ones: lane (g, c) gets
@@ -427,39 +636,34 @@ __device__ __forceinline__ void mma_3tf32(float (&d)[4], const uint32_t (&ah)[4]
   for (int e = 0; e < 4; ++e) d[e] += t[e];
 }
 
-__global__ void __launch_bounds__(kThreads) paged_f32(const Dev p, float* __restrict__ part) {
+__global__ void __launch_bounds__(kThreads, 8) paged_f32(const Dev p, float* __restrict__ part) {
   extern __shared__ __align__(128) uint8_t sm[];
-  float* qs = reinterpret_cast<float*>(sm + kWarps * kStages * kTile32);   // tf32 parts of the queries: hi rows, lo rows
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  float* qs = reinterpret_cast<float*>(sm + kStages * kTile32);   // the queries' rows
+  const int lane = threadIdx.x, g = lane >> 2, c = lane & 3;
   pdl_wait();
   pdl_trigger();
   Item it;
-  const bool any = item_of(p, &it);
-  const float* q = static_cast<const float*>(p.q) + it.b * p.sqb + it.h0 * p.sqh;
-  for (int r = 0; r < kRows; ++r) {
-    const float x = r < it.nh ? q[r * p.sqh + threadIdx.x] : 0.f;
-    uint32_t hi, lo;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
-    qs[r * kQPitch + threadIdx.x] = __uint_as_float(hi);
-    qs[(kRows + r) * kQPitch + threadIdx.x] = __uint_as_float(lo);
-  }
-  __syncthreads();
-  if (!any) {
+  if (!item_of(p, &it)) {
     if (it.len == 0) write_empty<float>(p, it);
     return;
   }
+  const float* q = static_cast<const float*>(p.q) + it.b * p.sqb + it.h0 * p.sqh + lane * 4;
+#pragma unroll 4
+  for (int r = 0; r < kRows; ++r)
+    *reinterpret_cast<float4*>(qs + r * kQPitch + lane * 4) =
+        r < it.nh ? *reinterpret_cast<const float4*>(q + r * p.sqh) : make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncwarp();
   const uint32_t sq = smem_u32(qs) + ((lane & 15) * kQPitch + (lane >> 4) * 4) * 4;   // matrices: rows 0-7, 8-15, then columns 4-7
   State st;
-  run_tiles<float>(p, it, smem_u32(sm) + warp * kStages * kTile32, part, st, [&](uint32_t K, uint32_t valid) {
+  run_tiles<float>(p, it, smem_u32(sm), part, st, [&](uint32_t K, uint32_t valid) {
     const uint32_t V = K + kKeys * kD * 4;
     float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     const int kr = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll 4
     for (int kk = 0; kk < kD / 8; ++kk) {
-      uint32_t ah[4], al[4], kb[4], kh[4], kl[4];
-      ldsm4(sq + kk * 32, ah);
-      ldsm4(sq + kRows * kQPitch * 4 + kk * 32, al);
+      uint32_t qb[4], ah[4], al[4], kb[4], kh[4], kl[4];
+      ldsm4(sq + kk * 32, qb);
+      split4(qb, ah, al);
       ldsm4(K + kr * (kD * 4) + (((kk * 2 + (lane >> 3 & 1)) ^ (kr & 7)) * 16), kb);
       split4(kb, kh, kl);
       mma_3tf32(sc[0], ah, al, kh[0], kh[1], kl[0], kl[1]);
@@ -567,6 +771,16 @@ static int paged_validate(const rb_paged_args* a) {
   return RB_OK;
 }
 
+// [pages, HK, page_size, 128] bf16 in boxes of one tile's 64 dims.
+static int page_map(CUtensorMap* m, const void* base, const rb_paged_args* a, int64_t slot, int64_t head, int64_t page) {
+  // a dimension of one entry may have any stride: give the map a plain one
+  const uint64_t dims[4] = {pg::kD, static_cast<uint64_t>(a->page_size), static_cast<uint64_t>(a->HK), static_cast<uint64_t>(a->pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(slot) * 2, static_cast<uint64_t>(a->HK > 1 ? head : 8) * 2,
+                               static_cast<uint64_t>(a->pages > 1 ? page : 8) * 2};
+  const uint32_t box[4] = {64, pg::kKeys, 1, 1};
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 size_t paged_workspace(const rb_paged_args* a) {
   if (paged_validate(a) != RB_OK || a->B == 0) return 0;
   const int splits = pg::max_chunks(paged_max_len(a));
@@ -593,14 +807,24 @@ int paged_launch(const rb_paged_args* a, void* ws, size_t ws_bytes, cudaStream_t
   // A warp takes one chunk while that leaves no more than about four rounds of warps, and
   // up to eight so that the ring's start is paid less often. No result depends on it.
   const int64_t chunks = static_cast<int64_t>(p.splits) * a->HK * tiles * a->B;
-  const int64_t rounds = chunks / (static_cast<int64_t>(device_sm_count()) * 2 * kWarps * 4);
+  const int64_t rounds = chunks / (static_cast<int64_t>(device_sm_count()) * 8 * 4);
   p.per_warp = static_cast<int>(rounds < 1 ? 1 : rounds > 8 ? 8 : rounds);
-  const dim3 grid((p.splits + kWarps * p.per_warp - 1) / (kWarps * p.per_warp), a->HK * tiles, a->B);
+  const dim3 grid((p.splits + p.per_warp - 1) / p.per_warp, a->HK * tiles, a->B);
   const bool bf = a->dtype == RB_BF16;
-  const int smem = bf ? smem16() : smem32();
-  if (cudaFuncSetAttribute(bf ? paged_bf16 : paged_f32, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return RB_ERR_CUDA;
-  r = launch_k(bf ? paged_bf16 : paged_f32, grid, dim3(kThreads), smem, st, true, p, part);
+  auto go = [&](auto kern, int smem, auto&&... args) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return static_cast<int>(RB_ERR_CUDA);
+    return launch_k(kern, grid, dim3(kThreads), smem, st, true, args..., p, part);
+  };
+  if (bf) {
+    CUtensorMap tk{}, tv{};
+    const bool tma = a->page_size % kKeys == 0 && a->pages > 0 && page_map(&tk, a->k, a, a->sks, a->skh, a->skp) == RB_OK &&
+                     page_map(&tv, a->v, a, a->svs, a->svh, a->svp) == RB_OK;   // rows gathered one by one where a map cannot say it
+    const bool one = a->H / a->HK <= 8;
+    r = one ? (tma ? go(paged_bf16<1, true>, smem16(), tk, tv) : go(paged_bf16<1, false>, smem16(), tk, tv))
+            : (tma ? go(paged_bf16<2, true>, smem16(), tk, tv) : go(paged_bf16<2, false>, smem16(), tk, tv));
+  } else {
+    r = go(paged_f32, smem32());
+  }
   if (r != RB_OK || p.splits == 1) return r;
   return launch_k(bf ? join_chunks<uint16_t> : join_chunks<float>, dim3(a->H, a->B), dim3(32 * kJoinWarps), 0, st, true, p,
                   static_cast<const float*>(part));
