@@ -13,8 +13,10 @@
 // bf16: S^T = K Q^T and O^T = V^T P^T on m16n8k16 tiles, so that the group's heads are the
 // 8 (or 16) columns: a group of up to 8 wastes no rows and needs half the accumulators. P
 // enters as two bf16 parts (hi + lo), so a weight is good to 2^-16 and the result is
-// rounded once, at the end. Where pages hold whole tiles, a tile is four TMA boxes. fp32:
-// three tf32 products per term, each step from zero and added in fp32.
+// rounded once, at the end. fp32: three tf32 products per term, each step from zero and
+// added in fp32. Where pages hold whole tiles, a tile arrives as TMA boxes, else row by row.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_util.h"
 
@@ -24,36 +26,34 @@ namespace pg {
 constexpr int kD = 128;
 constexpr int kThreads = 32;               // a block is one warp: they share nothing, and spread evenly
 constexpr int kKeys = 16;                  // keys of a tile
-#ifndef RULE
-#define RULE 2
-#endif
-constexpr int kStages = 3;
+constexpr int kStages = 3;                 // tiles in a warp's ring; eight warps an SM
 constexpr int kRows = 16;                  // query heads of a block
 constexpr int kMinChunk = 32, kMaxChunk = 2048;
 
-// Keys per chunk of a sequence of `len` tokens: 64 up to 4,096 tokens, then doubled each
-// time the length is four times larger. A chunk's result costs G x 520 bytes written and
-// read against 512 bytes a key (bf16): 6% of the traffic for a group of 4 at 64.
-__host__ __device__ inline int chunk_of(int len) {
-  int c = kMinChunk;
-  while (c < kMaxChunk && static_cast<int64_t>(RULE) * c * c < len) c *= 2;
+// Keys per chunk of a sequence of `len` tokens: in bf16 64 up to 4,096 tokens, then doubled
+// each time the length is four times larger; in fp32, whose keys are twice as long and cost
+// several times the instructions, 32 up to 16,384. A chunk's result costs G x 520 bytes written and read against 512 bytes a key
+// (bf16): 6% of the traffic for a group of 4 at 64.
+__host__ __device__ constexpr int kGrow(int es) { return es == 2 ? 1 : 16; }
+__host__ __device__ inline int chunk_of(int len, int es) {
+  int c = kMinChunk * 4 / es;
+  while (c < kMaxChunk && static_cast<int64_t>(kGrow(es)) * c * c < len) c *= 2;
   return c;
 }
-__host__ __device__ inline int chunks_of(int len) {
-  const int c = chunk_of(len);
+__host__ __device__ inline int chunks_of(int len, int es) {
+  const int c = chunk_of(len, es);
   return len / c + (len % c != 0);
 }
 // Upper bound of chunks_of over every length up to `len`.
-__host__ inline int max_chunks(int len) {
+__host__ inline int max_chunks(int len, int es) {
   int n = 1;
-  for (int c = kMinChunk; c <= kMaxChunk; c *= 2) {   // the longest length each size serves
-    const int64_t top = c < kMaxChunk ? static_cast<int64_t>(RULE) * c * c : len;
+  for (int c = kMinChunk * 4 / es;; c *= 2) {   // the longest length each size serves
+    const int64_t top = c < kMaxChunk ? static_cast<int64_t>(kGrow(es)) * c * c : len;
     const int x = static_cast<int>(top < len ? top : len);
-    const int k = chunks_of(x);
+    const int k = chunks_of(x, es);
     n = k > n ? k : n;
-    if (x == len) break;
+    if (x == len) return n;
   }
-  return n;
 }
 
 struct Dev {
@@ -64,6 +64,7 @@ struct Dev {
   const int32_t *table, *lengths, *seqs;
   int64_t ld_table;
   int B, H, HK, pages, page_size, width, rows, ahead, max_len;
+  int es;                                  // bytes of an element
   int splits, per_warp;                    // chunks a sequence may have; consecutive chunks a warp takes
   void* out;
   int64_t sob, soh;
@@ -78,13 +79,6 @@ __device__ __forceinline__ int length_of(const Dev& p, int b, int* row) {
   const int64_t len = static_cast<int64_t>(p.lengths[r]) + p.ahead;
   return static_cast<int>(len < 0 ? 0 : len > p.max_len ? p.max_len : len);
 }
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes < 16: zero fill
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -112,47 +106,14 @@ __device__ __forceinline__ bool item_of(const Dev& p, Item* it) {
   int row;
   it->len = length_of(p, it->b, &row);
   it->table = p.table + row * p.ld_table;
-  it->chunk = chunk_of(it->len);
-  it->chunks = chunks_of(it->len);
+  it->chunk = chunk_of(it->len, p.es);
+  it->chunks = chunks_of(it->len, p.es);
   it->c0 = blockIdx.x * p.per_warp;
   if (it->c0 >= it->chunks) return false;
   it->k0 = it->c0 * it->chunk;
   it->k1 = min(static_cast<int64_t>(it->len), it->k0 + static_cast<int64_t>(p.per_warp) * it->chunk);
   return true;
 }
-// The page of this lane's key (lane & 15) of tile t, -1 where there is none: its token is left out.
-__device__ __forceinline__ int page_of(const Dev& p, const Item& it, int t) {
-  const int key = it.k0 + t * kKeys + (threadIdx.x & 15);
-  if (key >= it.k1) return -1;
-  const int x = it.table[key / p.page_size];
-  return x < p.pages ? x : -1;
-}
-
-// Copies tile t's K and V rows (RB bytes each) into `dst` (K rows, then V rows; 16-byte
-// pieces swizzled by row & 7); rows without a page become zeros. Returns which of the
-// tile's keys there are.
-template <int RB>
-__device__ __forceinline__ uint32_t fetch(const Dev& p, const Item& it, int t, int page, uint32_t dst) {
-  constexpr int P = RB / 16, R = 32 / P;   // pieces of a row, rows of one pass
-  constexpr int es = RB / kD;
-  const int lane = threadIdx.x & 31, piece = lane % P;
-  const int slot = (it.k0 + t * kKeys + (lane & 15)) % p.page_size;
-  const int64_t ko = page < 0 ? 0 : (page * p.skp + slot * p.sks) * es, vo = page < 0 ? 0 : (page * p.svp + slot * p.svs) * es;
-  const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
-  const uint8_t* k = static_cast<const uint8_t*>(p.k) + it.kvh * p.skh * es + piece * 16;
-  const uint8_t* v = static_cast<const uint8_t*>(p.v) + it.kvh * p.svh * es + piece * 16;
-#pragma unroll
-  for (int i = 0; i < kKeys / R; ++i) {
-    const int row = i * R + lane / P;
-    const int64_t a = __shfl_sync(0xffffffffu, ko, row), b = __shfl_sync(0xffffffffu, vo, row);
-    const uint32_t n = (valid >> row & 1) ? 16u : 0u;
-    const uint32_t at = dst + row * RB + ((piece ^ (row & 7)) * 16);
-    copy16(at, n ? k + a : p.q, n);        // a row that does not exist reads nothing
-    copy16(at + kKeys * RB, n ? v + b : p.q, n);
-  }
-  return valid;
-}
-
 // Where a chunk's result goes: accumulators [B, H, splits, kD], then (max, sum) [B, H, splits].
 __device__ __forceinline__ float* acc_at(const Dev& p, float* part, const Item& it, int r, int c) {
   return part + ((static_cast<int64_t>(it.b) * p.H + it.h0 + r) * p.splits + c) * kD;
@@ -212,147 +173,20 @@ __device__ __noinline__ void redo_row(const Dev& p, const Item& it, float* part,
   }
 }
 
-// A finished chunk: fragments of rows g, g + 8 (columns 8 n + 2 c, + 1), their maxima and
-// this lane's share of their sums.
-template <typename T>
-__device__ __forceinline__ void finish(const Dev& p, const Item& it, float* part, int chunk, const float (&o)[kD / 8][4],
-                                       const float (&m)[2], const float (&l)[2]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float s = l[h];
-    s += __shfl_xor_sync(0xffffffffu, s, 1);
-    s += __shfl_xor_sync(0xffffffffu, s, 2);
-    const int r = g + h * 8;
-    bool nan = false;
-    if (r < it.nh) {
-      if (it.chunks == 1) {
-        const float inv = s > 0.f || s != s ? 1.f : 0.f;   // no token at all: zeros
-        const float div = inv == 0.f ? 1.f : s;
-#pragma unroll
-        for (int n = 0; n < kD / 8; ++n) {
-          const float a = o[n][h * 2] / div * inv, b = o[n][h * 2 + 1] / div * inv;
-          nan |= a != a || b != b;
-          if (sizeof(T) == 4) *reinterpret_cast<float2*>(out_at<float>(p, it, r) + n * 8 + c * 2) = make_float2(a, b);
-          else *reinterpret_cast<uint32_t*>(out_at<uint16_t>(p, it, r) + n * 8 + c * 2) = pack_bf16x2(a, b);
-        }
-      } else {
-        float* dst = acc_at(p, part, it, r, chunk);
-#pragma unroll
-        for (int n = 0; n < kD / 8; ++n) {
-          nan |= o[n][h * 2] != o[n][h * 2] || o[n][h * 2 + 1] != o[n][h * 2 + 1];
-          *reinterpret_cast<float2*>(dst + n * 8 + c * 2) = make_float2(o[n][h * 2], o[n][h * 2 + 1]);
-        }
-        if (c == 0) *ml_at(p, part, it, r, chunk) = make_float2(m[h], s);
-      }
-    }
-    unsigned again = __ballot_sync(0xffffffffu, nan);
-    for (int x = 0; again; ++x, again >>= 4)
-      if (again & 0xFu) redo_row<T>(p, it, part, h * 8 + x, chunk);   // the four lanes of row x
-  }
-}
-
-constexpr int kTile16 = 2 * kKeys * kD * 2, kTile32 = 2 * kKeys * kD * 4;
-constexpr int kQPitch = kD + 4;            // floats per staged fp32 query row: ldmatrix without bank conflicts
-constexpr int smem16() { return 1024 + kStages * kTile16 + 64; }   // ring, mbarriers
-constexpr int smem32() { return kStages * kTile32 + kRows * kQPitch * 4; }
-static_assert(smem32() <= 232448, "shared memory budget");
-
-// The running state of one warp's 16 rows, and what a tile does to it.
-struct State {
-  float o[kD / 8][4], m[2], l[2];
-  __device__ __forceinline__ void reset() {
-#pragma unroll
-    for (int n = 0; n < kD / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
-  }
-  // Scores of two 8-key tiles become weights; O is rescaled where a maximum moves.
-  __device__ __forceinline__ void weigh(float (&sc)[2][4], uint32_t valid, float scale2) {
-    const int c = threadIdx.x & 3;
-    float alpha[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {   // rows g and g + 8
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = sc[j][h * 2 + e];
-          x = (valid >> (j * 8 + c * 2 + e) & 1) ? x * scale2 : -INFINITY;
-          mx = fmaxf(mx, x);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      mx = fmaxf(mx, m[h]);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      alpha[h] = fast_exp2(m[h] - ref);
-      m[h] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = sc[j][h * 2 + e];
-          x = fast_exp2(x - ref);
-          sum += x;
-        }
-      l[h] = fmaf(l[h], alpha[h], sum);
-    }
-    if (!__all_sync(0xffffffffu, alpha[0] == 1.f && alpha[1] == 1.f)) {
-#pragma unroll
-      for (int n = 0; n < kD / 8; ++n) {
-        o[n][0] *= alpha[0];
-        o[n][1] *= alpha[0];
-        o[n][2] *= alpha[1];
-        o[n][3] *= alpha[1];
-      }
-    }
+// A tile in shared memory, K then V. From TMA boxes: blocks of 128 bytes of all 16 rows,
+// 16-byte pieces swizzled by row & 7. Gathered: whole rows, 16 bytes apart beyond their
+// length. Either way eight rows' pieces of one column lie in different banks.
+constexpr int kQPitch = kD + 4;
+template <typename T, bool kTma>
+struct Ring {
+  static constexpr int kRow = kD * sizeof(T);
+  static constexpr int kSide = kKeys * (kTma ? kRow : kRow + 16), kTile = 2 * kSide;
+  // ring, mbarriers, fp32: the tile's weights and the queries (pitches free of bank conflicts)
+  static constexpr int kSmem = 1024 + kStages * kTile + 64 + (sizeof(T) == 4 ? (kKeys * 20 + kRows * kQPitch) * 4 : 0);
+  __device__ __forceinline__ static uint32_t at(uint32_t side, int row, int piece) {
+    return kTma ? side + (piece >> 3) * (kKeys * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16) : side + row * (kRow + 16) + piece * 16;
   }
 };
-
-// Runs a warp's tiles through its ring: `use(K)` after tile t has arrived at K.
-template <typename T, typename Use>
-__device__ __forceinline__ void run_tiles(const Dev& p, const Item& it, uint32_t ring, float* part, State& st, Use use) {
-  constexpr int kTile = sizeof(T) == 2 ? kTile16 : kTile32, RB = kD * sizeof(T);
-  const int tiles = (it.k1 - it.k0 + kKeys - 1) / kKeys, per_chunk = it.chunk / kKeys;
-  uint32_t valid[kStages];
-  int page = page_of(p, it, 0);            // of the next tile to fetch, looked up one tile ahead
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    valid[s] = s < tiles ? fetch<RB>(p, it, s, page, ring + s * kTile) : 0;
-    page = page_of(p, it, s + 1);
-    copy_commit();
-  }
-  st.reset();
-  int left = per_chunk, chunk = it.c0;
-  for (int t0 = 0; t0 < tiles; t0 += kStages) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) {
-      const int t = t0 + s;
-      if (t >= tiles) break;
-      constexpr int kAhead = kStages - 1;
-      const int sn = (s + kAhead) % kStages;   // the stage read last
-      valid[sn] = t + kAhead < tiles ? fetch<RB>(p, it, t + kAhead, page, ring + sn * kTile) : 0;
-      page = page_of(p, it, t + kAhead + 1);
-      copy_commit();
-      copy_wait<kAhead>();
-      __syncwarp();
-      use(ring + s * kTile, valid[s]);
-      __syncwarp();                            // the stage has been read before it is filled again
-      if (--left == 0 || t + 1 == tiles) {
-        finish<T>(p, it, part, chunk++, st.o, st.m, st.l);
-        st.reset();
-        left = per_chunk;
-      }
-    }
-  }
-}
-
-// ---------------------------------------------------------------- bf16
-constexpr int kHalf16 = kKeys * 128;       // 64 dims of a tile's rows: 128 bytes each, 16-byte pieces swizzled by row & 7
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int slot, int head, int page) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
@@ -365,19 +199,59 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {   // an 8 x 8 bf16 
   return r;
 }
 
+// x = hi + lo: hi rounded to tf32's 11 bits by integer arithmetic (the conversion
+// instruction is several times slower), lo what is left, which the tensor core cuts to 11
+// bits: good to 2^-22 of x. A NaN survives in lo; an infinity gives one.
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+struct Split4 {
+  uint32_t hi[4], lo[4];
+  __device__ __forceinline__ explicit Split4(const uint32_t (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split(__uint_as_float(x[e]), hi[e], lo[e]);
+  }
+};
+struct Split2 {
+  uint32_t hi[2], lo[2];
+  __device__ __forceinline__ Split2(float a, float b) {
+    split(a, hi[0], lo[0]);
+    split(b, hi[1], lo[1]);
+  }
+};
+__device__ __forceinline__ void mma_3tf32(float (&d)[4], const Split4& a, const Split2& b) {
+  float t[4] = {0.f, 0.f, 0.f, 0.f};   // the tensor core's own additions truncate: keep them short
+  mma_tf32(t, a.lo, b.hi[0], b.hi[1]);
+  mma_tf32(t, a.hi, b.lo[0], b.lo[1]);
+  mma_tf32(t, a.hi, b.hi[0], b.hi[1]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d[e] += t[e];
+}
+
 // NT: columns of 8 query heads. kTma: pages hold whole tiles (page size % 16 == 0), so a tile
 // lies in one page; else its rows are gathered one by one.
-template <int NT, bool kTma>
+template <typename T, int NT, bool kTma>
 __global__ void __launch_bounds__(kThreads, 8)
-    paged_bf16(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Dev p,
+    paged_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Dev p,
                float* __restrict__ part) {
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x, g = lane >> 2, c = lane & 3;
-  const uint32_t ring = smem_u32(sm), bars = ring + kStages * kTile16;
-  if (kTma && lane == 0) {
-    tma_prefetch_desc(&tk);
-    tma_prefetch_desc(&tv);
+  using R = Ring<T, kTma>;
+  constexpr int kTile = R::kTile, kSide = R::kSide, kPieces = R::kRow / 16;
+  const uint32_t ring = smem_u32(sm), bars = ring + kStages * kTile;
+  if (lane == 0) {
+    if (kTma) {
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
+    }
     for (int i = 0; i < kStages; ++i) mbar_init(bars + i * 8, 1);
     fence_mbar_init();
   }
@@ -386,72 +260,87 @@ __global__ void __launch_bounds__(kThreads, 8)
   pdl_trigger();
   Item it;
   if (!item_of(p, &it)) {
-    if (it.len == 0) write_empty<uint16_t>(p, it);
+    if (it.len == 0) write_empty<T>(p, it);
     return;
   }
   const int tiles = (it.k1 - it.k0 + kKeys - 1) / kKeys, per_chunk = it.chunk / kKeys;
   // the page of tile t (kTma: of the tile; else of this lane's key), looked up one tile ahead
   auto page_at = [&](int t) {
-    if (!kTma) return page_of(p, it, t);
-    if (t >= tiles) return -1;
-    const int x = it.table[(it.k0 + t * kKeys) / p.page_size];
-    return x < p.pages ? x : -1;
+    const int key = it.k0 + t * kKeys + (kTma ? 0 : lane & 15);
+    if (key >= it.k1) return -1;
+    const int x = it.table[key / p.page_size];
+    return x < p.pages ? x : -1;           // -1: no page, its tokens are left out
   };
   auto get = [&](int t, int page, int stage) -> uint32_t {   // starts tile t; which of its keys there are
-    const uint32_t dst = ring + stage * kTile16;
+    const uint32_t dst = ring + stage * kTile;
     const int key = it.k0 + t * kKeys;
+    const uint32_t bar = bars + stage * 8;
+    const int n = it.k1 - key;
     if (kTma) {
       if (lane == 0) {
-        const uint32_t bar = bars + stage * 8;
         if (page >= 0) {
           const int slot = key % p.page_size;
-          mbar_arrive_expect_tx(bar, kTile16);
-          tma_box(dst, &tk, bar, 0, slot, it.kvh, page);
-          tma_box(dst + kHalf16, &tk, bar, 64, slot, it.kvh, page);
-          tma_box(dst + 2 * kHalf16, &tv, bar, 0, slot, it.kvh, page);
-          tma_box(dst + 3 * kHalf16, &tv, bar, 64, slot, it.kvh, page);
+          mbar_arrive_expect_tx(bar, kTile);
+#pragma unroll
+          for (int x = 0; x < R::kRow / 128; ++x) {
+            tma_box(dst + x * kKeys * 128, &tk, bar, x * 128 / sizeof(T), slot, it.kvh, page);
+            tma_box(dst + kSide + x * kKeys * 128, &tv, bar, x * 128 / sizeof(T), slot, it.kvh, page);
+          }
         } else {
           mbar_arrive(bar);
         }
       }
-      const int n = it.k1 - key;
       return page < 0 ? 0u : n < kKeys ? (1u << n) - 1u : 0xFFFFu;
     }
-    const int slot = (key + (lane & 15)) % p.page_size, piece = lane & 15;
-    const int64_t ko = page < 0 ? 0 : page * p.skp + slot * p.sks, vo = page < 0 ? 0 : page * p.svp + slot * p.svs;
+    // a row a lane: the lower sixteen fetch K, the others V; rows that do not exist become zeros
     const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0) & 0xFFFFu;
-    const uint16_t* k = static_cast<const uint16_t*>(p.k) + it.kvh * p.skh + piece * 8;
-    const uint16_t* v = static_cast<const uint16_t*>(p.v) + it.kvh * p.svh + piece * 8;
-#pragma unroll
-    for (int i = 0; i < kKeys / 2; ++i) {
-      const int row = i * 2 + (lane >> 4);
-      const int64_t a = __shfl_sync(0xffffffffu, ko, row), b = __shfl_sync(0xffffffffu, vo, row);
-      const bool ok = valid >> row & 1;
-      const uint32_t at = dst + (piece >> 3) * kHalf16 + row * 128 + (((piece & 7) ^ (row & 7)) * 16);
-      copy16(at, ok ? static_cast<const void*>(k + a) : p.q, ok ? 16u : 0u);   // a row that does not exist reads nothing
-      copy16(at + 2 * kHalf16, ok ? static_cast<const void*>(v + b) : p.q, ok ? 16u : 0u);
+    const int row = lane & 15, slot = (key + row) % p.page_size;
+    const uint32_t to = dst + (lane >> 4) * kSide + row * (R::kRow + 16);
+    if (page < 0) {
+      for (int x = 0; x < kPieces; ++x) asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(to + x * 16), "r"(0) : "memory");
+      fence_proxy_async_smem();   // a later copy may land here
+    }
+    if (lane == 0) mbar_arrive_expect_tx(bar, __popc(valid) * 2 * R::kRow);
+    __syncwarp();
+    if (page >= 0) {
+      const T* from = lane < 16 ? static_cast<const T*>(p.k) + page * p.skp + it.kvh * p.skh + slot * p.sks
+                                : static_cast<const T*>(p.v) + page * p.svp + it.kvh * p.svh + slot * p.svs;
+      bulk_load(to, from, R::kRow, bar);
     }
     return valid;
   };
 
-  uint32_t valid[kStages];
+  constexpr int kPitch = NT == 1 ? 12 : 20;   // fp32 weights, [key][head]: free of bank conflicts
+  float* weights = reinterpret_cast<float*>(sm + kStages * kTile + 64);
+  uint32_t* queries = reinterpret_cast<uint32_t*>(weights + kKeys * 20);
+  // which keys there are of tiles t, t + 1 and t + 2
+  static_assert(kStages == 3, "live, live1, live2");
   int page = page_at(0);
+  uint32_t live = get(0, page, 0);
+  page = page_at(1);
+  uint32_t live1 = tiles > 1 ? get(1, page, 1) : 0, live2 = 0;
+  page = page_at(2);
+  // Queries as B fragments: column g of each eight (heads past the group are zero). A step
+  // is 32 bytes of a row: 16 bf16 or 8 fp32; either way lane c has bytes 4 c and 16 + 4 c.
+  // fp32 has them in shared memory.
+  constexpr int kSteps = kD * sizeof(T) / 32;
+  const uint32_t* q = static_cast<const uint32_t*>(p.q) + (it.b * p.sqb + it.h0 * p.sqh) * sizeof(T) / 4;
+  uint32_t qb[NT][sizeof(T) == 2 ? kSteps : 1][2];
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    valid[s] = s < tiles ? get(s, page, s) : 0;
-    page = page_at(s + 1);
-    if (!kTma) copy_commit();
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int kk = 0; kk < kSteps; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qb[n][kk][e] = n * 8 + g < it.nh ? q[(n * 8 + g) * p.sqh / 2 + kk * 8 + e * 4 + c] : 0u;
+  } else {
+#pragma unroll 4
+    for (int r = 0; r < NT * 8; ++r)
+      *reinterpret_cast<uint4*>(queries + r * kQPitch + lane * 4) =
+          r < it.nh ? *reinterpret_cast<const uint4*>(q + r * p.sqh + lane * 4) : make_uint4(0, 0, 0, 0);
+    __syncwarp();
   }
-  // queries as B fragments: column g of each eight (heads past the group are zero)
-  uint32_t qb[NT][kD / 16][2];
-  const uint16_t* q = static_cast<const uint16_t*>(p.q) + it.b * p.sqb + it.h0 * p.sqh;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int kk = 0; kk < kD / 16; ++kk)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        qb[n][kk][e] = n * 8 + g < it.nh ? *reinterpret_cast<const uint32_t*>(q + (n * 8 + g) * p.sqh + kk * 16 + e * 8 + c * 2) : 0u;
   // O^T: rows = dims 16 d + g, + 8; columns = heads 8 n + 2 c, + 1, as are m and l (l: this lane's keys)
   float o[kD / 16][NT][4], m[NT][2], l[NT][2];
   auto reset = [&] {
@@ -469,48 +358,50 @@ __global__ void __launch_bounds__(kThreads, 8)
   int left = per_chunk, chunk = it.c0;
   uint32_t phase = 0;
   for (int t0 = 0; t0 < tiles; t0 += kStages, phase ^= 1) {
-#pragma unroll
+#pragma unroll(sizeof(T) == 2 ? kStages : 1)   // fp32 has code enough as it is
     for (int s = 0; s < kStages; ++s) {
       const int t = t0 + s;
       if (t >= tiles) break;
       constexpr int kAhead = kStages - 1;
-      const int sn = (s + kAhead) % kStages;   // the stage read last
-      valid[sn] = t + kAhead < tiles ? get(t + kAhead, page, sn) : 0;
+      live2 = t + kAhead < tiles ? get(t + kAhead, page, s == 0 ? kAhead : s - 1) : 0;   // into the stage read last
       page = page_at(t + kAhead + 1);
-      const uint32_t K = ring + s * kTile16, V = K + 2 * kHalf16, live = valid[s];
-      if (kTma) {
-        if (!__all_sync(0xffffffffu, mbar_wait_spin(bars + s * 8, phase, 0x321))) {   // an error flag is up: see the copies out
-          for (int x = t; x < min(tiles, t + kStages); ++x) mbar_wait(bars + x % kStages * 8, x / kStages & 1, 0x321);
-          return;
-        }
-        if (live != 0xFFFFu && live != 0u) {
-          // slots past the last token hold whatever was there: zero weights would not silence it
-          const int n = __popc(live);
-          for (int x = lane; x < kKeys * 16; x += 32)
-            if ((x >> 4) >= n)
-              asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(V + ((x >> 3) & 1) * kHalf16 + (x >> 4) * 128 + (x & 7) * 16), "r"(0) : "memory");
-        }
-      } else {
-        copy_commit();
-        copy_wait<kAhead>();
+      const uint32_t K = ring + s * kTile, V = K + kSide;
+      if (!__all_sync(0xffffffffu, mbar_wait_spin(bars + s * 8, phase, 0x321))) {   // an error flag is up: see the copies out
+        for (int x = t; x < min(tiles, t + kStages); ++x) mbar_wait(bars + x % kStages * 8, x / kStages & 1, 0x321);
+        return;
+      }
+      if (kTma && live != 0xFFFFu && live != 0u) {
+        // slots past the last token hold whatever was there: zero weights would not silence it
+        const int n = __popc(live);
+        for (int x = lane; x < kKeys * kPieces; x += 32)
+          if (x / kPieces >= n)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(R::at(V, x / kPieces, x % kPieces)), "r"(0) : "memory");
       }
       __syncwarp();
       if (live) {   // the same in every lane
-        float sc[NT][4];
+        float sc[NT][4], odd[NT][4];   // bf16: the odd steps apart, which halves the chain of dependent products
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) sc[n][e] = odd[n][e] = 0.f;
         const int kr = lane & 15;                                   // ldmatrix rows: keys 0-7, 8-15, then the next 8 dims
-#pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
+#pragma unroll(sizeof(T) == 2 ? kSteps : 4)
+        for (int kk = 0; kk < kSteps; ++kk) {   // ldmatrix moves 8 x 4 fp32 blocks as it moves 8 x 8 bf16 ones
           uint32_t a[4];
-          const int piece = kk * 2 + (lane >> 4);
-          ldsm4(K + (piece >> 3) * kHalf16 + kr * 128 + (((piece & 7) ^ (kr & 7)) * 16), a);
+          ldsm4(R::at(K, kr, kk * 2 + (lane >> 4)), a);
+          if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_bf16_16816(sc[n], a[0], a[1], a[2], a[3], qb[n][kk][0], qb[n][kk][1]);
+            for (int n = 0; n < NT; ++n) mma_bf16_16816(kk & 1 ? odd[n] : sc[n], a[0], a[1], a[2], a[3], qb[n][kk][0], qb[n][kk][1]);
+          } else {
+            const Split4 as(a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint32_t* qr = queries + (n * 8 + g) * kQPitch + kk * 8 + c;
+              mma_3tf32(sc[n], as, Split2(__uint_as_float(qr[0]), __uint_as_float(qr[4])));
+            }
+          }
         }
-        uint32_t hi[NT][2], lo[NT][2];
+        uint32_t hi[NT][2], lo[NT][2];   // bf16 weights as B fragments, in two parts
         float alpha[NT][2];
         bool same = true;
 #pragma unroll
@@ -519,8 +410,8 @@ __global__ void __launch_bounds__(kThreads, 8)
           for (int e = 0; e < 2; ++e) {   // column 2 c + e: this lane has keys g and g + 8
             float& x = sc[n][e];
             float& y = sc[n][2 + e];
-            x = (live >> g & 1) ? x * p.scale2 : -INFINITY;
-            y = (live >> (g + 8) & 1) ? y * p.scale2 : -INFINITY;
+            x = (live >> g & 1) ? (x + odd[n][e]) * p.scale2 : -INFINITY;
+            y = (live >> (g + 8) & 1) ? (y + odd[n][2 + e]) * p.scale2 : -INFINITY;
             float mx = fmaxf(x, y);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
@@ -532,6 +423,12 @@ __global__ void __launch_bounds__(kThreads, 8)
             x = fast_exp2(x - ref);
             y = fast_exp2(y - ref);
             l[n][e] = fmaf(l[n][e], alpha[n][e], x + y);
+          }
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              *reinterpret_cast<float2*>(weights + (g + h * 8) * kPitch + n * 8 + c * 2) = make_float2(sc[n][2 * h], sc[n][2 * h + 1]);
+            continue;
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {   // keys g, then g + 8: rows of an 8 x 8 matrix, turned into columns
@@ -549,17 +446,39 @@ __global__ void __launch_bounds__(kThreads, 8)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[d][n][e] *= alpha[n][e & 1];
         }
-        const int vr = (lane & 7) + (lane >> 4) * 8;                // ldmatrix rows: keys 0-7 (dims 0-7, 8-15), keys 8-15
+        if constexpr (sizeof(T) == 2) {
+          const int vr = (lane & 7) + (lane >> 4) * 8;              // ldmatrix rows: keys 0-7 (dims 0-7, 8-15), keys 8-15
 #pragma unroll
-        for (int d = 0; d < kD / 16; ++d) {
-          uint32_t a[4];
-          const int piece = d * 2 + (lane >> 3 & 1);
-          ldsm4_t(V + (piece >> 3) * kHalf16 + vr * 128 + (((piece & 7) ^ (vr & 7)) * 16), a);
+          for (int d = 0; d < kD / 16; ++d) {
+            uint32_t a[4];
+            ldsm4_t(R::at(V, vr, d * 2 + (lane >> 3 & 1)), a);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
-            mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
+              mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+            }
           }
+        } else {
+          // The order of a step's eight keys is free: keys 2 c and 2 c + 1 serve as columns c
+          // and c + 4, which reads V without bank conflicts.
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float* w = weights + (j * 8 + c * 2) * kPitch + n * 8 + g;
+              const Split2 ws(w[0], w[kPitch]);
+#pragma unroll
+              for (int d = 0; d < kD / 16; ++d) {
+                uint32_t a[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {   // (dim g, key 2c), (g + 8, 2c), (g, 2c + 1), (g + 8, 2c + 1)
+                  const int dim = d * 16 + g + (e & 1) * 8;
+                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(a[e]) : "r"(R::at(V, j * 8 + c * 2 + (e >> 1), dim >> 2) + (dim & 3) * 4));
+                }
+                mma_3tf32(o[d][n], Split4(a), ws);
+              }
+            }
         }
         __syncwarp();                      // the stage has been read before it is filled again
       }
@@ -576,14 +495,15 @@ __global__ void __launch_bounds__(kThreads, 8)
             if (r < it.nh) {
               if (it.chunks == 1) {
                 const bool some = sum > 0.f || sum != sum;   // no token at all: zeros
-                uint16_t* dst = out_at<uint16_t>(p, it, r) + g;
+                T* dst = out_at<T>(p, it, r) + g;
 #pragma unroll
                 for (int d = 0; d < kD / 16; ++d)
 #pragma unroll
                   for (int h = 0; h < 2; ++h) {
                     const float y = some ? o[d][n][h * 2 + e] / sum : 0.f;
                     nan |= y != y;
-                    dst[d * 16 + h * 8] = f32_to_bf16_bits(y);
+                    if constexpr (sizeof(T) == 2) dst[d * 16 + h * 8] = f32_to_bf16_bits(y);
+                    else dst[d * 16 + h * 8] = y;
                   }
               } else {
                 float* dst = acc_at(p, part, it, r, chunk) + g;
@@ -600,97 +520,17 @@ __global__ void __launch_bounds__(kThreads, 8)
             const unsigned again = __ballot_sync(0xffffffffu, nan);
             if (again) {
               for (int x = 0; x < 4; ++x)
-                if (again & (0x11111111u << x)) redo_row<uint16_t>(p, it, part, n * 8 + x * 2 + e, chunk);
+                if (again & (0x11111111u << x)) redo_row<T>(p, it, part, n * 8 + x * 2 + e, chunk);
             }
           }
         reset();
         left = per_chunk;
         ++chunk;
       }
+      live = live1;
+      live1 = live2;
     }
   }
-}
-
-// fp32. ldmatrix moves 8 x 4 fp32 blocks as it moves 8 x 8 bf16 ones: lane (g, c) gets
-// row g, column c, which is what a tf32 fragment wants of Q and of K.
-__device__ __forceinline__ void split4(const uint32_t (&x)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi[e]) : "f"(__uint_as_float(x[e])));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo[e]) : "f"(__uint_as_float(x[e]) - __uint_as_float(hi[e])));
-  }
-}
-__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_3tf32(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t h0, uint32_t h1,
-                                          uint32_t l0, uint32_t l1) {
-  float t[4] = {0.f, 0.f, 0.f, 0.f};   // the tensor core's own additions truncate: keep them short
-  mma_tf32(t, al, h0, h1);
-  mma_tf32(t, ah, l0, l1);
-  mma_tf32(t, ah, h0, h1);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) d[e] += t[e];
-}
-
-__global__ void __launch_bounds__(kThreads, 8) paged_f32(const Dev p, float* __restrict__ part) {
-  extern __shared__ __align__(128) uint8_t sm[];
-  float* qs = reinterpret_cast<float*>(sm + kStages * kTile32);   // the queries' rows
-  const int lane = threadIdx.x, g = lane >> 2, c = lane & 3;
-  pdl_wait();
-  pdl_trigger();
-  Item it;
-  if (!item_of(p, &it)) {
-    if (it.len == 0) write_empty<float>(p, it);
-    return;
-  }
-  const float* q = static_cast<const float*>(p.q) + it.b * p.sqb + it.h0 * p.sqh + lane * 4;
-#pragma unroll 4
-  for (int r = 0; r < kRows; ++r)
-    *reinterpret_cast<float4*>(qs + r * kQPitch + lane * 4) =
-        r < it.nh ? *reinterpret_cast<const float4*>(q + r * p.sqh) : make_float4(0.f, 0.f, 0.f, 0.f);
-  __syncwarp();
-  const uint32_t sq = smem_u32(qs) + ((lane & 15) * kQPitch + (lane >> 4) * 4) * 4;   // matrices: rows 0-7, 8-15, then columns 4-7
-  State st;
-  run_tiles<float>(p, it, smem_u32(sm), part, st, [&](uint32_t K, uint32_t valid) {
-    const uint32_t V = K + kKeys * kD * 4;
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    const int kr = (lane & 7) + (lane >> 4) * 8;
-#pragma unroll 4
-    for (int kk = 0; kk < kD / 8; ++kk) {
-      uint32_t qb[4], ah[4], al[4], kb[4], kh[4], kl[4];
-      ldsm4(sq + kk * 32, qb);
-      split4(qb, ah, al);
-      ldsm4(K + kr * (kD * 4) + (((kk * 2 + (lane >> 3 & 1)) ^ (kr & 7)) * 16), kb);
-      split4(kb, kh, kl);
-      mma_3tf32(sc[0], ah, al, kh[0], kh[1], kl[0], kl[1]);
-      mma_3tf32(sc[1], ah, al, kh[2], kh[3], kl[2], kl[3]);
-    }
-    st.weigh(sc, valid, p.scale2);
-    // the order of a step's eight keys is free: the accumulator's columns (2c, 2c + 1)
-    // serve as the A fragment's (c, c + 4), and V's rows follow
-    uint32_t ph[2][4], pl[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t x[4] = {__float_as_uint(sc[j][0]), __float_as_uint(sc[j][2]), __float_as_uint(sc[j][1]), __float_as_uint(sc[j][3])};
-      split4(x, ph[j], pl[j]);
-    }
-#pragma unroll
-    for (int n = 0; n < kD / 8; ++n) {
-      uint32_t x[4], vh[4], vl[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = (e >> 1) * 8 + c * 2 + (e & 1);
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[e]) : "r"(V + key * (kD * 4) + (((n * 2 + (g >> 2)) ^ (key & 7)) * 16) + (g & 3) * 4));
-      }
-      split4(x, vh, vl);
-      mma_3tf32(st.o[n], ph[0], pl[0], vh[0], vh[1], vl[0], vl[1]);
-      mma_3tf32(st.o[n], ph[1], pl[1], vh[2], vh[3], vl[2], vl[3]);
-    }
-  });
 }
 
 // Block (head, sequence): warp w takes chunks w, w + kJoinWarps, ..., four dims a lane; the
@@ -704,7 +544,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks(const Dev p, cons
   pdl_trigger();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int row;
-  const int n = chunks_of(length_of(p, b, &row));
+  const int n = chunks_of(length_of(p, b, &row), p.es);
   if (n <= 1) return;   // written by the chunk's own warp
   const int64_t head = (static_cast<int64_t>(b) * p.H + h) * p.splits;
   const float4* acc = reinterpret_cast<const float4*>(part + head * kD) + lane;
@@ -771,19 +611,21 @@ static int paged_validate(const rb_paged_args* a) {
   return RB_OK;
 }
 
-// [pages, HK, page_size, 128] bf16 in boxes of one tile's 64 dims.
+// [pages, HK, page_size, 128] in boxes of 128 bytes of one tile's rows.
 static int page_map(CUtensorMap* m, const void* base, const rb_paged_args* a, int64_t slot, int64_t head, int64_t page) {
+  const uint32_t es = a->dtype == RB_BF16 ? 2 : 4;
   // a dimension of one entry may have any stride: give the map a plain one
   const uint64_t dims[4] = {pg::kD, static_cast<uint64_t>(a->page_size), static_cast<uint64_t>(a->HK), static_cast<uint64_t>(a->pages)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(slot) * 2, static_cast<uint64_t>(a->HK > 1 ? head : 8) * 2,
-                               static_cast<uint64_t>(a->pages > 1 ? page : 8) * 2};
-  const uint32_t box[4] = {64, pg::kKeys, 1, 1};
-  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t strides[3] = {static_cast<uint64_t>(slot) * es, static_cast<uint64_t>(a->HK > 1 ? head : 8) * es,
+                               static_cast<uint64_t>(a->pages > 1 ? page : 8) * es};
+  const uint32_t box[4] = {128 / es, pg::kKeys, 1, 1};
+  return encode_tiled(m, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 size_t paged_workspace(const rb_paged_args* a) {
   if (paged_validate(a) != RB_OK || a->B == 0) return 0;
-  const int splits = pg::max_chunks(paged_max_len(a));
+  const int splits = pg::max_chunks(paged_max_len(a), a->dtype == RB_BF16 ? 2 : 4);
   return splits > 1 ? static_cast<size_t>(a->B) * a->H * splits * (pg::kD + 2) * sizeof(float) : 0;
 }
 
@@ -799,7 +641,9 @@ int paged_launch(const rb_paged_args* a, void* ws, size_t ws_bytes, cudaStream_t
   p.v = a->v; p.svp = a->svp; p.svh = a->svh; p.svs = a->svs;
   p.table = a->table; p.lengths = a->lengths; p.seqs = a->seqs; p.ld_table = a->ld_table;
   p.B = a->B; p.H = a->H; p.HK = a->HK; p.pages = a->pages; p.page_size = a->page_size; p.width = a->width;
-  p.rows = a->rows; p.ahead = a->ahead; p.max_len = paged_max_len(a); p.splits = max_chunks(p.max_len);
+  p.rows = a->rows; p.ahead = a->ahead; p.max_len = paged_max_len(a);
+  p.es = a->dtype == RB_BF16 ? 2 : 4;
+  p.splits = max_chunks(p.max_len, p.es);
   p.out = a->out; p.sob = a->sob; p.soh = a->soh;
   p.scale2 = a->sm_scale * 1.4426950408889634f;
   float* part = static_cast<float*>(ws);
@@ -810,21 +654,23 @@ int paged_launch(const rb_paged_args* a, void* ws, size_t ws_bytes, cudaStream_t
   const int64_t rounds = chunks / (static_cast<int64_t>(device_sm_count()) * 8 * 4);
   p.per_warp = static_cast<int>(rounds < 1 ? 1 : rounds > 8 ? 8 : rounds);
   const dim3 grid((p.splits + p.per_warp - 1) / p.per_warp, a->HK * tiles, a->B);
-  const bool bf = a->dtype == RB_BF16;
-  auto go = [&](auto kern, int smem, auto&&... args) {
+  CUtensorMap tk{}, tv{};
+  // rows are gathered one by one where a tile may cross pages or a map cannot say the layout
+  const bool tma = a->page_size % kKeys == 0 && a->pages > 0 && page_map(&tk, a->k, a, a->sks, a->skh, a->skp) == RB_OK &&
+                   page_map(&tv, a->v, a, a->svs, a->svh, a->svp) == RB_OK;
+  auto go = [&](auto kern, int smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return static_cast<int>(RB_ERR_CUDA);
-    return launch_k(kern, grid, dim3(kThreads), smem, st, true, args..., p, part);
+    return launch_k(kern, grid, dim3(kThreads), smem, st, true, tk, tv, p, part);
   };
-  if (bf) {
-    CUtensorMap tk{}, tv{};
-    const bool tma = a->page_size % kKeys == 0 && a->pages > 0 && page_map(&tk, a->k, a, a->sks, a->skh, a->skp) == RB_OK &&
-                     page_map(&tv, a->v, a, a->svs, a->svh, a->svp) == RB_OK;   // rows gathered one by one where a map cannot say it
-    const bool one = a->H / a->HK <= 8;
-    r = one ? (tma ? go(paged_bf16<1, true>, smem16(), tk, tv) : go(paged_bf16<1, false>, smem16(), tk, tv))
-            : (tma ? go(paged_bf16<2, true>, smem16(), tk, tv) : go(paged_bf16<2, false>, smem16(), tk, tv));
-  } else {
-    r = go(paged_f32, smem32());
-  }
+  const bool bf = a->dtype == RB_BF16, one = a->H / a->HK <= 8;
+  auto both = [&](auto zero, auto nt) {
+    using T = decltype(zero);
+    constexpr int NT = decltype(nt)::value;
+    return tma ? go(paged_kernel<T, NT, true>, Ring<T, true>::kSmem) : go(paged_kernel<T, NT, false>, Ring<T, false>::kSmem);
+  };
+  const std::integral_constant<int, 1> nt1{};
+  const std::integral_constant<int, 2> nt2{};
+  r = bf ? (one ? both(uint16_t(0), nt1) : both(uint16_t(0), nt2)) : (one ? both(0.f, nt1) : both(0.f, nt2));
   if (r != RB_OK || p.splits == 1) return r;
   return launch_k(bf ? join_chunks<uint16_t> : join_chunks<float>, dim3(a->H, a->B), dim3(32 * kJoinWarps), 0, st, true, p,
                   static_cast<const float*>(part));

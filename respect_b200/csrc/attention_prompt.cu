@@ -139,14 +139,12 @@ constexpr int kPitch = kD + 4;   // floats per staged row: fragment reads withou
 constexpr int kTile = kKeys * kPitch;
 constexpr int kSmem = (kRows * kPitch + 4 * kTile) * 4;
 
-__device__ __forceinline__ uint32_t tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
+// x = hi + lo: hi rounded to tf32's 11 bits by integer arithmetic (the conversion
+// instruction is several times slower), lo what is left, which the tensor core cuts to 11
+// bits: good to 2^-22 of x. A NaN survives in lo; an infinity gives one.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  hi = tf32(x);
-  lo = tf32(x - __uint_as_float(hi));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(

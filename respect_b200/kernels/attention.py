@@ -146,9 +146,9 @@ def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_bytes(B: int, H: int, HK: int, page_size: int, width: int, max_length: int) -> int:
+def _paged_bytes(dtype: int, B: int, H: int, HK: int, page_size: int, width: int, max_length: int) -> int:
     """Scratch of a paged call: a function of its sizes."""
-    a = _lib.PagedArgs(dtype=_lib.RB_BF16, B=B, H=H, HK=HK, D=128, page_size=page_size, width=width, ld_table=width,
+    a = _lib.PagedArgs(dtype=dtype, B=B, H=H, HK=HK, D=128, page_size=page_size, width=width, ld_table=width,
                        max_length=max_length, q=16, out=16, lengths=16, table=16)
     return _lib.lib().rb_paged_attn_workspace(ctypes.byref(a))
 
@@ -186,12 +186,13 @@ def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=Non
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), y.stride()
     pages, HK, page_size, _ = k.shape
     bound = int(max_length or 0)
-    a = _lib.pack_paged_args(_lib.dtype_code(q.dtype), B, H, HK, D, q.data_ptr(), sq[0], sq[1],
+    dtype = _lib.dtype_code(q.dtype)
+    a = _lib.pack_paged_args(dtype, B, H, HK, D, q.data_ptr(), sq[0], sq[1],
                              k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], pages, page_size,
                              table.data_ptr(), max(table.stride(0), width), width, rows, lengths.data_ptr(),
                              seqs.data_ptr() if seqs is not None else 0, ahead, bound, y.data_ptr(), so[0], so[1],
                              D ** -0.5 if sm_scale is None else sm_scale)
-    nbytes = _paged_bytes(B, H, HK, page_size, width, bound)
+    nbytes = _paged_bytes(dtype, B, H, HK, page_size, width, bound)
     ws = _lib.scratch(q, nbytes)
     _lib.launch("rb_paged_attn", q, a, ws.data_ptr() if ws is not None else None, nbytes)
     return y
