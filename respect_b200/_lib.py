@@ -195,12 +195,13 @@ def launch(name: str, t: torch.Tensor, *args) -> None:
     dev = t.get_device()
     if dev < 0:
         raise ValueError("respect_b200 operators take CUDA tensors (no CPU path)")
-    st = torch._C._cuda_getCurrentRawStream(dev)   # torch.cuda.current_stream without the Stream object
-    if dev == torch._C._cuda_getDevice():
-        call(name, *args, st)
-    else:
+    stream = torch._C._cuda_getCurrentRawStream(dev)   # torch.cuda.current_stream without the Stream object
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            call(name, *args, st)
+            return call(name, *args, stream)
+    status = getattr(_lib or lib(), name)(*args, stream)
+    if status != RB_OK:
+        raise RespectNativeError(name, status, lib().rb_status_string(status).decode())
 
 
 def scratch(t: torch.Tensor, nbytes: int) -> torch.Tensor | None:

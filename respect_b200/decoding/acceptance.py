@@ -49,32 +49,34 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
     [offset, offset + size) excluded as in greedy_token (-inf for an excluded token; excluded
     entries follow the others among the alternatives). A row holding NaN or +inf, or nothing but
     -inf, gives NaN, and so does a token outside the vocabulary."""
-    if logits.dim() == 0 or logits.dtype not in (torch.float32, torch.bfloat16):
+    shape, dtype = logits.shape, logits.dtype
+    if not shape or (dtype is not torch.float32 and dtype is not torch.bfloat16):
         raise TypeError("token_logprobs takes fp32 or bf16 logits [..., vocab]")
-    V = logits.shape[-1]
-    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1] or tokens.device != logits.device:
-        raise ValueError(f"tokens must be int64 {tuple(logits.shape[:-1])} on {logits.device}")
+    V, lead = shape[-1], shape[:-1]
+    if tokens.dtype is not torch.int64 or tokens.shape != lead or tokens.get_device() != logits.get_device():
+        raise ValueError(f"tokens must be int64 {tuple(lead)} on {logits.device}")
     if not 0 <= top <= min(_lib.LOGPROBS_MAX_TOP, V):
         raise ValueError(f"top must be between 0 and {min(_lib.LOGPROBS_MAX_TOP, V)}")
     if offset < 0 or size < 0 or V == 0:
         raise ValueError("token_logprobs: bad excluded range or empty vocabulary")
-    x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
-    lead = x.shape[:-1]
-    if x.dim() != 2:
+    x = logits if V == 1 or logits.stride(-1) == 1 else logits.contiguous()
+    if len(lead) != 1:
         x, tokens = x.reshape(-1, V), tokens.reshape(-1)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     M, dev = x.shape[0], x.device
-    out = torch.empty((2 + top) * M, dtype=torch.float32, device=dev)
-    ids = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
-    lp, ent = out[:M], out[M:2 * M]
-    tlp = out[2 * M:].view(*lead, top) if top else None
+    if top:
+        lp, ent, tlp = torch.empty((2 + top) * M, dtype=torch.float32, device=dev).split_with_sizes((M, M, top * M))
+        tlp, ids = tlp.view(*lead, top), torch.empty((*lead, top), dtype=torch.int64, device=dev)
+        tlp_at, ids_at = tlp.data_ptr(), ids.data_ptr()
+    else:
+        lp, ent = torch.empty(2 * M, dtype=torch.float32, device=dev).split_with_sizes((M, M))
+        tlp = ids = tlp_at = ids_at = None
     nbytes = _scratch_bytes(M, V, top)
     ws = _lib.scratch(x, nbytes)
-    _lib.launch("rb_token_logprobs", x, x.data_ptr(), _lib.dtype_code(x.dtype), x.stride(0) if M > 1 else V, M, V,
-                tokens.data_ptr(), min(offset, V), min(size, V), top, lp.data_ptr(), ent.data_ptr(),
-                tlp.data_ptr() if top else None, ids.data_ptr() if top else None,
-                ws.data_ptr() if ws is not None else None, nbytes)
+    _lib.launch("rb_token_logprobs", x, x.data_ptr(), _lib.dtype_code(dtype), x.stride(0) if M > 1 else V, M, V,
+                tokens.data_ptr(), min(offset, V), min(size, V), top, lp.data_ptr(), ent.data_ptr(), tlp_at, ids_at,
+                None if ws is None else ws.data_ptr(), nbytes)
     if len(lead) != 1:
         lp, ent = lp.view(lead), ent.view(lead)
     return TokenLogprobs(lp, ent, tlp, ids)

@@ -29,6 +29,7 @@ import ctypes
 import torch
 
 from respect_b200 import _lib
+from respect_b200.kernels.attention import _rows as rows
 from respect_b200.kernels.attention import paged_attention
 
 STATUS = {1: "a sequence that does not exist, is named twice, or is a fork's target in use",
@@ -83,7 +84,7 @@ class PagedKVCache:
         if not store.is_contiguous():
             raise ValueError("store must be contiguous")
         self.store, self.table, self.lengths, self.held, self.refs = store, table, lengths, held, refs
-        self.device, self.dtype = store.device, store.dtype
+        self.device, self.dtype, self._dev = store.device, store.dtype, store.get_device()
         self.layers, _, self.pages, self.kv_heads, self.page_size, self.head_dim = store.shape
         self.max_seqs, self.max_pages = table.shape
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -101,11 +102,12 @@ class PagedKVCache:
     def _list(self, x, name: str, n: int | None = None) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
             x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
-        if x.dtype != torch.int32 or x.device != self.device or x.dim() != 1:
+        if x.dtype is not torch.int32 or x.get_device() != self._dev or x.dim() != 1:
             raise TypeError(f"{name} must be a list or an int32 tensor of one dimension on {self.device}")
-        if n is not None and x.numel() != n:
-            raise ValueError(f"{name} holds {x.numel()} entries, expected {n}")
-        if x.numel() > _lib.PAGES_MAX_LIST:
+        m = x.numel()
+        if n is not None and m != n:
+            raise ValueError(f"{name} holds {m} entries, expected {n}")
+        if m > _lib.PAGES_MAX_LIST:
             raise ValueError(f"{name}: at most {_lib.PAGES_MAX_LIST} sequences per call")
         return x if x.is_contiguous() else x.contiguous()
 
@@ -125,34 +127,29 @@ class PagedKVCache:
         """K and V of new tokens to the positions after the committed ones, inside reserved room:
         tokens [offsets[i], offsets[i + 1]) belong to seqs[i] (default: one token each). k, v
         [tokens, kv_heads, head_dim] for one ``layer``, [layers, tokens, kv_heads, head_dim] for all."""
-        dims = 4 if layer is None else 3
         s = self._list(seqs, "seqs")
-        n = s.numel()
-        for name, t in (("k", k), ("v", v)):
-            if t.dim() != dims or t.dtype != self.dtype or t.device != self.device:
-                raise ValueError(f"{name} must be a {self.dtype} tensor of {dims} dimensions on {self.device}")
-            if tuple(t.shape[-2:]) != (self.kv_heads, self.head_dim) or (layer is None and t.shape[0] != self.layers):
-                raise ValueError(f"{name} {tuple(t.shape)} does not fit the cache")
-        if k.shape != v.shape:
-            raise ValueError("k and v must share a shape")
+        n, ks = s.numel(), k.shape
+        want = (self.layers,) if layer is None else ()
+        if len(ks) != 3 + len(want) or ks != v.shape or ks[:-3] != want or ks[-2:] != (self.kv_heads, self.head_dim):
+            raise ValueError(f"k {tuple(ks)}, v {tuple(v.shape)} do not fit: expected "
+                             f"[{'layers, ' if layer is None else ''}tokens, {self.kv_heads}, {self.head_dim}]")
         if layer is not None and not 0 <= layer < self.layers:
             raise IndexError(f"layer {layer} of {self.layers}")
-        if offsets is None and k.shape[-3] != n:
-            raise ValueError(f"{k.shape[-3]} tokens for {n} sequences: pass offsets")
-        if offsets is not None:
+        T = ks[-3]
+        if offsets is None:
+            if T != n:
+                raise ValueError(f"{T} tokens for {n} sequences: pass offsets")
+        else:
             if not isinstance(offsets, torch.Tensor):
                 offsets = torch.tensor(list(offsets), dtype=torch.int32, device=self.device)
-            if offsets.dtype != torch.int32 or offsets.device != self.device or tuple(offsets.shape) != (n + 1,):
+            if offsets.dtype is not torch.int32 or offsets.get_device() != self._dev or offsets.shape != (n + 1,):
                 raise ValueError(f"offsets must be int32 [{n + 1}] on {self.device}")
             offsets = offsets.contiguous()
-        unit = 16 // k.element_size()
-        k, v = (t if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(x % unit for x in t.stride()[:-1])
-                else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
-        lead = (lambda t: t.stride(0)) if layer is None else (lambda t: 0)
-        x = _lib.KVTokens(k.data_ptr(), v.data_ptr(), lead(k), k.stride(-3), k.stride(-2), lead(v), v.stride(-3),
-                          v.stride(-2), layer or 0, self.layers if layer is None else 1, k.shape[-3])
-        self._call("rb_kv_pages_write", ctypes.byref(x), s.data_ptr(), offsets.data_ptr() if offsets is not None else None,
-                   n)
+        k, v = rows(k, "k", self.store), rows(v, "v", self.store)
+        sk, sv = k.stride(), v.stride()
+        x = _lib.KVTokens(k.data_ptr(), v.data_ptr(), sk[0] if layer is None else 0, sk[-3], sk[-2],
+                          sv[0] if layer is None else 0, sv[-3], sv[-2], layer or 0, self.layers if layer is None else 1, T)
+        self._call("rb_kv_pages_write", ctypes.byref(x), s.data_ptr(), None if offsets is None else offsets.data_ptr(), n)
 
     def commit(self, seqs, counts) -> None:
         """The next counts[i] written tokens of seqs[i] belong to it."""

@@ -80,23 +80,21 @@ def fused_attn_hyb(q, kp, vp, kn, vn, msk, sm_scale=None,
 
 def _laid_out(t: torch.Tensor) -> bool:
     """Unit inner stride, everything else in whole 16-byte pieces."""
-    st = t.stride()
-    odd = 0
-    for x in st[:-1]:
-        odd |= x                     # a negative stride cannot occur; any low bit set shows
-    return st[-1] == 1 and odd % (16 // t.element_size()) == 0 and t.data_ptr() % 16 == 0
+    *outer, inner = t.stride()
+    odd = t.data_ptr() // t.element_size()
+    for x in outer:
+        odd |= x                     # any low bit set shows
+    return inner == 1 and odd % (16 // t.element_size()) == 0
 
 
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     """t with the layout the kernels read; a copy only if it lacks it."""
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
     return t if _laid_out(t) else t.clone(memory_format=torch.contiguous_format)
 
 
-def _out(out, q: torch.Tensor) -> torch.Tensor:
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+def _out(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
     if not _laid_out(out):
@@ -104,19 +102,19 @@ def _out(out, q: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _int32(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != dims:
-        raise TypeError(f"{name} must be an int32 tensor of {dims} dimension(s) on {device}")
+def _int32(t: torch.Tensor, name: str, dims: int, like: torch.Tensor) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != like.get_device() or t.dim() != dims:
+        raise TypeError(f"{name} must be an int32 tensor of {dims} dimension(s) on {like.device}")
     return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
 
 
-def _check_heads(q: torch.Tensor, heads_kv: int, dim: int) -> None:
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError(f"attention takes bf16 or fp32, got {q.dtype}")
-    if dim != 128 or q.shape[-1] != 128:
+def _check_heads(dtype: torch.dtype, heads: int, heads_kv: int, dim: int, dim_kv: int) -> None:
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise TypeError(f"attention takes bf16 or fp32, got {dtype}")
+    if dim != 128 or dim_kv != 128:
         raise ValueError("attention heads must have 128 dims")
-    if heads_kv == 0 or q.shape[1] == 0 or q.shape[1] % heads_kv:
-        raise ValueError(f"{q.shape[1]} query heads do not share {heads_kv} kv heads evenly")
+    if heads_kv == 0 or heads == 0 or heads % heads_kv:
+        raise ValueError(f"{heads} query heads do not share {heads_kv} kv heads evenly")
 
 
 def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
@@ -126,21 +124,24 @@ def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
     read in place), cu_seqlens int32 [B + 1] on the same device: sequence i is tokens
     [cu_seqlens[i], cu_seqlens[i + 1]), ascending. Returns [T, H, 128]. Rows of no
     sequence are zero in a new result and left as they were in a given ``out``."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0]:
-        raise ValueError(f"prompt_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
-    _check_heads(q, k.shape[1], k.shape[2])
-    if q.shape[1] // k.shape[1] > 64:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[0] != qs[0]:
+        raise ValueError(f"prompt_attention: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} do not fit")
+    T, H, D = qs
+    HK = ks[1]
+    _check_heads(q.dtype, H, HK, D, ks[2])
+    if H > 64 * HK:
         raise ValueError("prompt_attention: at most 64 query heads per kv head")
-    cu = _int32(cu_seqlens, "cu_seqlens", 1, q.device)
-    if cu.numel() < 1:
+    cu = _int32(cu_seqlens, "cu_seqlens", 1, q)
+    B = cu.numel() - 1
+    if B < 0:
         raise ValueError("cu_seqlens holds one entry more than there are sequences")
     q, k, v = _rows(q, "q", q), _rows(k, "k", q), _rows(v, "v", q)
-    y = _out(out, q)
-    T, H, D = q.shape
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _out(out, q)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), y.stride()
-    a = _lib.pack_prompt_args(_lib.dtype_code(q.dtype), cu.numel() - 1, T, H, k.shape[1], D, q.data_ptr(), sq[0], sq[1],
-                              k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], cu.data_ptr(),
-                              y.data_ptr(), so[0], so[1], D ** -0.5 if sm_scale is None else sm_scale, out is None)
+    a = _lib.pack_prompt_args(_lib.dtype_code(q.dtype), B, T, H, HK, D, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1],
+                              v.data_ptr(), sv[0], sv[1], cu.data_ptr(), y.data_ptr(), so[0], so[1],
+                              D ** -0.5 if sm_scale is None else sm_scale, out is None)
     _lib.launch("rb_prompt_attn", q, a)
     return y
 
@@ -163,12 +164,13 @@ def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=Non
     row (``ahead`` counts tokens written but not committed yet), cut to the table's
     width and to ``max_length``, a bound on the lengths that keeps scratch and launch
     small when the table is much wider. No tokens give zeros. Returns [B, H, 128]."""
-    if q.dim() != 3 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise ValueError(f"paged_attention: q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)}, "
-                         f"v_pages {tuple(v_pages.shape)} do not fit")
-    _check_heads(q, k_pages.shape[1], k_pages.shape[3])
-    B, H, D = q.shape
-    table, lengths = _int32(table, "table", 2, q.device), _int32(lengths, "lengths", 1, q.device)
+    qs, ks = q.shape, k_pages.shape
+    if len(qs) != 3 or len(ks) != 4 or ks != v_pages.shape:
+        raise ValueError(f"paged_attention: q {tuple(qs)}, k_pages {tuple(ks)}, v_pages {tuple(v_pages.shape)} do not fit")
+    B, H, D = qs
+    pages, HK, page_size, dim = ks
+    _check_heads(q.dtype, H, HK, D, dim)
+    table, lengths = _int32(table, "table", 2, q), _int32(lengths, "lengths", 1, q)
     rows, width = table.shape
     if lengths.numel() != rows:
         raise ValueError(f"{lengths.numel()} lengths for {rows} table rows")
@@ -176,23 +178,22 @@ def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=Non
         if rows != B:
             raise ValueError(f"{rows} table rows for {B} queries: name the rows with seqs")
     else:
-        seqs = _int32(seqs, "seqs", 1, q.device)
+        seqs = _int32(seqs, "seqs", 1, q)
         if seqs.numel() != B:
             raise ValueError(f"{seqs.numel()} seqs for {B} queries")
     if ahead < 0 or (max_length is not None and max_length < 1):
         raise ValueError("ahead must not be negative, max_length must be positive")
     q, k, v = _rows(q, "q", q), _rows(k_pages, "k_pages", q), _rows(v_pages, "v_pages", q)
-    y = _out(out, q)
+    y = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else _out(out, q)
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), y.stride()
-    pages, HK, page_size, _ = k.shape
-    bound = int(max_length or 0)
+    bound = max_length or 0
     dtype = _lib.dtype_code(q.dtype)
-    a = _lib.pack_paged_args(dtype, B, H, HK, D, q.data_ptr(), sq[0], sq[1],
-                             k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], pages, page_size,
-                             table.data_ptr(), max(table.stride(0), width), width, rows, lengths.data_ptr(),
-                             seqs.data_ptr() if seqs is not None else 0, ahead, bound, y.data_ptr(), so[0], so[1],
+    a = _lib.pack_paged_args(dtype, B, H, HK, D, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], sk[2],
+                             v.data_ptr(), sv[0], sv[1], sv[2], pages, page_size, table.data_ptr(),
+                             max(table.stride(0), width), width, rows, lengths.data_ptr(),
+                             0 if seqs is None else seqs.data_ptr(), ahead, bound, y.data_ptr(), so[0], so[1],
                              D ** -0.5 if sm_scale is None else sm_scale)
     nbytes = _paged_bytes(dtype, B, H, HK, page_size, width, bound)
     ws = _lib.scratch(q, nbytes)
-    _lib.launch("rb_paged_attn", q, a, ws.data_ptr() if ws is not None else None, nbytes)
+    _lib.launch("rb_paged_attn", q, a, None if ws is None else ws.data_ptr(), nbytes)
     return y
