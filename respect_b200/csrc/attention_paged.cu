@@ -26,7 +26,6 @@ namespace pg {
 constexpr int kD = 128;
 constexpr int kThreads = 32;               // a block is one warp: they share nothing, and spread evenly
 constexpr int kKeys = 16;                  // keys of a tile
-constexpr int kStages = 3;                 // tiles in a warp's ring; eight warps an SM
 constexpr int kRows = 16;                  // query heads of a block
 constexpr int kMinChunk = 32, kMaxChunk = 2048;
 
@@ -179,6 +178,7 @@ __device__ __noinline__ void redo_row(const Dev& p, const Item& it, float* part,
 constexpr int kQPitch = kD + 4;
 template <typename T, bool kTma>
 struct Ring {
+  static constexpr int kStages = sizeof(T) == 2 ? 3 : 2;   // tiles in a warp's ring: eight bf16 warps an SM, five fp32
   static constexpr int kRow = kD * sizeof(T);
   static constexpr int kSide = kKeys * (kTma ? kRow : kRow + 16), kTile = 2 * kSide;
   // ring, mbarriers, fp32: the tile's weights and the queries (pitches free of bank conflicts)
@@ -207,7 +207,7 @@ __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(   // not volatile: independent products may pass one another
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -235,6 +235,12 @@ __device__ __forceinline__ void mma_3tf32(float (&d)[4], const Split4& a, const 
   for (int e = 0; e < 4; ++e) d[e] += t[e];
 }
 
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
 // NT: columns of 8 query heads. kTma: pages hold whole tiles (page size % 16 == 0), so a tile
 // lies in one page; else its rows are gathered one by one.
 template <typename T, int NT, bool kTma>
@@ -245,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 8)
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int lane = threadIdx.x, g = lane >> 2, c = lane & 3;
   using R = Ring<T, kTma>;
-  constexpr int kTile = R::kTile, kSide = R::kSide, kPieces = R::kRow / 16;
+  constexpr int kStages = R::kStages, kTile = R::kTile, kSide = R::kSide, kPieces = R::kRow / 16;
   const uint32_t ring = smem_u32(sm), bars = ring + kStages * kTile;
   if (lane == 0) {
     if (kTma) {
@@ -313,13 +319,13 @@ __global__ void __launch_bounds__(kThreads, 8)
   constexpr int kPitch = NT == 1 ? 12 : 20;   // fp32 weights, [key][head]: free of bank conflicts
   float* weights = reinterpret_cast<float*>(sm + kStages * kTile + 64);
   uint32_t* queries = reinterpret_cast<uint32_t*>(weights + kKeys * 20);
-  // which keys there are of tiles t, t + 1 and t + 2
-  static_assert(kStages == 3, "live, live1, live2");
+  uint32_t there[kStages];                 // which keys there are of tiles t, t + 1, ...
   int page = page_at(0);
-  uint32_t live = get(0, page, 0);
-  page = page_at(1);
-  uint32_t live1 = tiles > 1 ? get(1, page, 1) : 0, live2 = 0;
-  page = page_at(2);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    there[i] = i < tiles ? get(i, page, i) : 0;
+    page = page_at(i + 1);
+  }
   // Queries as B fragments: column g of each eight (heads past the group are zero). A step
   // is 32 bytes of a row: 16 bf16 or 8 fp32; either way lane c has bytes 4 c and 16 + 4 c.
   // fp32 has them in shared memory.
@@ -363,8 +369,9 @@ __global__ void __launch_bounds__(kThreads, 8)
       const int t = t0 + s;
       if (t >= tiles) break;
       constexpr int kAhead = kStages - 1;
-      live2 = t + kAhead < tiles ? get(t + kAhead, page, s == 0 ? kAhead : s - 1) : 0;   // into the stage read last
+      there[kAhead] = t + kAhead < tiles ? get(t + kAhead, page, s == 0 ? kAhead : s - 1) : 0;   // into the stage read last
       page = page_at(t + kAhead + 1);
+      const uint32_t live = there[0];
       const uint32_t K = ring + s * kTile, V = K + kSide;
       if (!__all_sync(0xffffffffu, mbar_wait_spin(bars + s * 8, phase, 0x321))) {   // an error flag is up: see the copies out
         for (int x = t; x < min(tiles, t + kStages); ++x) mbar_wait(bars + x % kStages * 8, x / kStages & 1, 0x321);
@@ -391,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 8)
           ldsm4(R::at(K, kr, kk * 2 + (lane >> 4)), a);
           if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16_16816(kk & 1 ? odd[n] : sc[n], a[0], a[1], a[2], a[3], qb[n][kk][0], qb[n][kk][1]);
+            for (int n = 0; n < NT; ++n) mma_bf16(kk & 1 ? odd[n] : sc[n], a, qb[n][kk]);
           } else {
             const Split4 as(a);
 #pragma unroll
@@ -454,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, 8)
             ldsm4_t(R::at(V, vr, d * 2 + (lane >> 3 & 1)), a);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], hi[n][0], hi[n][1]);
-              mma_bf16_16816(o[d][n], a[0], a[1], a[2], a[3], lo[n][0], lo[n][1]);
+              mma_bf16(o[d][n], a, hi[n]);
+              mma_bf16(o[d][n], a, lo[n]);
             }
           }
         } else {
@@ -527,8 +534,8 @@ __global__ void __launch_bounds__(kThreads, 8)
         left = per_chunk;
         ++chunk;
       }
-      live = live1;
-      live1 = live2;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) there[i] = there[i + 1];
     }
   }
 }

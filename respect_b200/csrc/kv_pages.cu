@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(256) copy_pages(const PagesDev s, const int32_
 }
 
 // ---------------------------------------------------------------- write
-// A warp per (token, layer): token t belongs to entry i with offsets[i] <= t <
+// A warp per token and `each` layers (finding the place costs several trips to memory, the
+// data one): token t belongs to entry i with offsets[i] <= t <
 // offsets[i + 1] (no offsets: t itself) and goes to position length + t - offsets[i].
 // Tokens before offsets[0] or from offsets[n] on belong to nobody.
 constexpr int kWriteWarps = 4;
@@ -207,7 +208,7 @@ struct WriteSrc {
 };
 __global__ void __launch_bounds__(32 * kWriteWarps)
     write_tokens(const PagesDev s, const WriteSrc k, const WriteSrc v, const int32_t* __restrict__ seqs,
-                 const int32_t* __restrict__ offsets, int n, int tokens, int layer0) {
+                 const int32_t* __restrict__ offsets, int n, int tokens, int layer0, int layers, int each) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -247,14 +248,31 @@ __global__ void __launch_bounds__(32 * kWriteWarps)
   const int vecs = s.row_bytes / 16, per = s.kv_heads * vecs;
   const int64_t head = static_cast<int64_t>(s.page_size) * vecs;
   const int64_t side = static_cast<int64_t>(s.pages) * s.kv_heads * head;
-  uint4* dst = reinterpret_cast<uint4*>(s.store) + static_cast<int64_t>(layer0 + blockIdx.y) * 2 * side +
-               static_cast<int64_t>(page) * s.kv_heads * head + (pos % s.page_size) * vecs;
-  const uint8_t* ks = k.p + blockIdx.y * k.s_layer + t * k.s_token;
-  const uint8_t* vs = v.p + blockIdx.y * v.s_layer + t * v.s_token;
-  for (int x = lane; x < per; x += 32) {
-    const int h = x / vecs, c = x % vecs;
-    dst[h * head + c] = *reinterpret_cast<const uint4*>(ks + h * k.s_head + c * 16);
-    dst[side + h * head + c] = *reinterpret_cast<const uint4*>(vs + h * v.s_head + c * 16);
+  uint4* dst0 = reinterpret_cast<uint4*>(s.store) + static_cast<int64_t>(page) * s.kv_heads * head + (pos % s.page_size) * vecs;
+  const int end = min(layers, (static_cast<int>(blockIdx.y) + 1) * each);
+  for (int layer = blockIdx.y * each; layer < end; ++layer) {
+    uint4* dst = dst0 + static_cast<int64_t>(layer0 + layer) * 2 * side;
+    const uint8_t* ks = k.p + layer * k.s_layer + t * k.s_token;
+    const uint8_t* vs = v.p + layer * v.s_layer + t * v.s_token;
+    for (int x0 = lane; x0 < per; x0 += 128) {   // up to eight loads before their stores
+      uint4 a[4], b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = x0 + e * 32, h = x / vecs, c = x % vecs;
+        if (x < per) {
+          a[e] = __ldcs(reinterpret_cast<const uint4*>(ks + h * k.s_head + c * 16));
+          b[e] = __ldcs(reinterpret_cast<const uint4*>(vs + h * v.s_head + c * 16));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = x0 + e * 32, h = x / vecs, c = x % vecs;
+        if (x < per) {
+          dst[h * head + c] = a[e];
+          dst[side + h * head + c] = b[e];
+        }
+      }
+    }
   }
 }
 
@@ -364,8 +382,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------- compact
-// Plan: block i checks entry i (every block checks the list) and counts the bad
-// ones in flags[0], which the launch zeroed.
+// Plan: block i checks entry i (every block checks the list) and says so in flags[i].
 __global__ void __launch_bounds__(256)
     compact_plan(const PagesDev s, const int32_t* __restrict__ seqs, const int32_t* __restrict__ paths, int64_t ld,
                  int width, const int32_t* __restrict__ counts, int n, int32_t* __restrict__ flags) {
@@ -375,7 +392,7 @@ __global__ void __launch_bounds__(256)
   if (!check_list(s, seqs, n, set)) {
     if (threadIdx.x == 0) {
       refuse(s, RB_PAGES_BAD_SEQUENCE);
-      atomicOr(flags, 1);
+      flags[blockIdx.x] = 1;
     }
     return;
   }
@@ -396,22 +413,28 @@ __global__ void __launch_bounds__(256)
     }
   bad = __syncthreads_or(bad);
   shared = __syncthreads_or(shared);
-  if (threadIdx.x == 0 && (bad || shared)) {
-    refuse(s, bad ? RB_PAGES_BAD_COUNT : RB_PAGES_SHARED);
-    atomicOr(flags, 1);
+  if (threadIdx.x == 0) {
+    flags[blockIdx.x] = bad || shared;
+    if (bad || shared) refuse(s, bad ? RB_PAGES_BAD_COUNT : RB_PAGES_SHARED);
   }
 }
+// Whether any entry's plan found fault; block-wide.
+__device__ __forceinline__ bool refused(const int32_t* flags, int n) {
+  int any = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) any |= flags[i];
+  return __syncthreads_or(any);
+}
 // Block (x, entry): thread = one 16-byte piece of one (layer, side, head); tokens in
-// ascending order, eight loads before their stores: a source lies at or after its
+// ascending order, sixteen loads before their stores: a source lies at or after its
 // target, and after every earlier target, so no store meets a later load's source.
 constexpr int kMoveThreads = 128;
 __global__ void __launch_bounds__(kMoveThreads)
     compact_move(const PagesDev s, const int32_t* __restrict__ seqs, const int32_t* __restrict__ paths, int64_t ld,
-                 const int32_t* __restrict__ counts, const int32_t* __restrict__ flags) {
+                 const int32_t* __restrict__ counts, int n, const int32_t* __restrict__ flags) {
   __shared__ int64_t from[kMoveThreads], to[kMoveThreads];   // offsets of a slot in a head's pages, in pieces
   pdl_wait();
   pdl_trigger();
-  if (flags[0]) return;
+  if (refused(flags, n)) return;
   const int seq = seqs[blockIdx.y], m = counts[blockIdx.y], len = s.lengths[seq];
   const int vecs = s.row_bytes / 16;
   const int64_t head = static_cast<int64_t>(s.page_size) * vecs, page = head * s.kv_heads;
@@ -431,24 +454,24 @@ __global__ void __launch_bounds__(kMoveThreads)
     }
     __syncthreads();
     if (!live) continue;
-    for (int e0 = 0; e0 < cnt; e0 += 8) {
-      uint4 val[8];
+    for (int e0 = 0; e0 < cnt; e0 += 16) {
+      uint4 val[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 16; ++e)
         if (e0 + e < cnt) val[e] = base[from[e0 + e]];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 16; ++e)
         if (e0 + e < cnt) base[to[e0 + e]] = val[e];
     }
   }
 }
 // Block i: the accepted tokens count, pages past them go back.
 __global__ void __launch_bounds__(256)
-    compact_finish(const PagesDev s, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts,
+    compact_finish(const PagesDev s, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int n,
                    const int32_t* __restrict__ flags) {
   pdl_wait();
   pdl_trigger();
-  if (flags[0]) return;
+  if (refused(flags, n)) return;
   const int seq = seqs[blockIdx.x], len = s.lengths[seq] + counts[blockIdx.x];
   const int keep = ceil_div(len, s.page_size), held = s.held[seq];
   release(s, seq, keep, held);
@@ -518,8 +541,11 @@ int kv_pages_write(const rb_kv_pages* a, const rb_kv_tokens* x, const int32_t* s
   if (!aligned16(x->k) || !aligned16(x->v)) return RB_ERR_UNSUPPORTED;
   const WriteSrc k{static_cast<const uint8_t*>(x->k), x->skl * es, x->skt * es, x->skh * es};
   const WriteSrc v{static_cast<const uint8_t*>(x->v), x->svl * es, x->svt * es, x->svh * es};
-  return launch_k(write_tokens, dim3(ceil_div(x->tokens, kWriteWarps), x->layers), dim3(32 * kWriteWarps), 0, st,
-                  true, s, k, v, seqs, offsets, n, x->tokens, x->layer0);
+  // about 32 warps an SM before a warp takes a second layer
+  const int64_t work = static_cast<int64_t>(x->tokens) * x->layers / (device_sm_count() * 32);
+  const int each = static_cast<int>(work < 1 ? 1 : work > 8 ? 8 : work);
+  return launch_k(write_tokens, dim3(ceil_div(x->tokens, kWriteWarps), ceil_div(x->layers, each)), dim3(32 * kWriteWarps), 0,
+                  st, true, s, k, v, seqs, offsets, n, x->tokens, x->layer0, x->layers, each);
 }
 
 int kv_pages_commit(const rb_kv_pages* a, const int32_t* seqs, const int32_t* counts, int n, cudaStream_t st) {
@@ -566,14 +592,13 @@ int kv_pages_compact(const rb_kv_pages* a, const int32_t* seqs, const int32_t* p
   if (!seqs || !counts || (width > 0 && !paths)) return RB_ERR_INVALID_ARG;
   if (!ws || bytes < kv_pages_workspace(a)) return RB_ERR_WORKSPACE;
   int32_t* flags = static_cast<int32_t*>(ws);
-  if (cudaMemsetAsync(flags, 0, sizeof(int32_t), st) != cudaSuccess) return RB_ERR_CUDA;
-  r = launch_k(compact_plan, dim3(n), dim3(256), 0, st, false, s, seqs, paths, ld, width, counts, n, flags);
+  r = launch_k(compact_plan, dim3(n), dim3(256), 0, st, true, s, seqs, paths, ld, width, counts, n, flags);
   if (r != RB_OK) return r;
   const int64_t pieces = static_cast<int64_t>(s.layers) * 2 * s.kv_heads * (s.row_bytes / 16);
   r = launch_k(compact_move, dim3(static_cast<unsigned>((pieces + kMoveThreads - 1) / kMoveThreads), n), dim3(kMoveThreads),
-               0, st, true, s, seqs, paths, ld, counts, flags);
+               0, st, true, s, seqs, paths, ld, counts, n, flags);
   if (r != RB_OK) return r;
-  return launch_k(compact_finish, dim3(n), dim3(256), 0, st, true, s, seqs, counts, flags);
+  return launch_k(compact_finish, dim3(n), dim3(256), 0, st, true, s, seqs, counts, n, flags);
 }
 
 }  // namespace rb
