@@ -266,7 +266,7 @@ RB_API int rb_compact_kv(void* const* k_layers, void* const* v_layers, int n_lay
  * t / page_size; refs[p] is the number of sequences that hold page p (0 = free).
  * All of it is caller-owned device memory, so calls are asynchronous and
  * capturable; calls on one cache must be ordered by the caller (one stream, or
- * events). Lists hold at most RB_PAGES_MAX_LIST entries and name a sequence
+ * events). At most 2^20 pages, 2^30 tokens per sequence, 16,384 layers. Lists hold at most RB_PAGES_MAX_LIST entries and name a sequence
  * once. A call that cannot be served as a whole changes nothing and sets
  * *status (first failure stands) to an rb_pages_status; of rb_kv_pages_write
  * only the tokens concerned are left out. No reference counterpart: its buffer

@@ -227,8 +227,10 @@ struct Split2 {
   }
 };
 __device__ __forceinline__ void mma_3tf32(float (&d)[4], const Split4& a, const Split2& b) {
-  float t[4] = {0.f, 0.f, 0.f, 0.f};   // the tensor core's own additions truncate: keep them short
-  mma_tf32(t, a.lo, b.hi[0], b.hi[1]);
+  float t[4];                          // from zero: the tensor core's own additions truncate, so they are kept short
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(t[0]), "=f"(t[1]), "=f"(t[2]), "=f"(t[3])
+      : "r"(a.lo[0]), "r"(a.lo[1]), "r"(a.lo[2]), "r"(a.lo[3]), "r"(b.hi[0]), "r"(b.hi[1]), "f"(0.f));
   mma_tf32(t, a.hi, b.lo[0], b.lo[1]);
   mma_tf32(t, a.hi, b.hi[0], b.hi[1]);
 #pragma unroll

@@ -152,12 +152,17 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma8_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // from zero
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma3(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
   uint32_t h0, l0, h1, l1;
   split(b0, h0, l0);
   split(b1, h1, l1);
-  float t[4] = {0.f, 0.f, 0.f, 0.f};   // the tensor core's own additions truncate: keep them short
-  mma8(t, al, h0, h1);
+  float t[4];                          // from zero: the tensor core's own additions truncate, so they are kept short
+  mma8_zero(t, al, h0, h1);
   mma8(t, ah, l0, l1);
   mma8(t, ah, h0, h1);
 #pragma unroll

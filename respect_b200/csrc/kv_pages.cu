@@ -132,7 +132,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (last && asking == s.refs[page]) page = -1;
   }
   const int cow = page >= 0;
-  const int fresh = i < n ? max(0, static_cast<int>((static_cast<int64_t>(len) + count + ps - 1) / ps) - held) : 0;
+  int fresh = i < n ? max(0, static_cast<int>((static_cast<int64_t>(len) + count + ps - 1) / ps) - held) : 0;
+  fresh = min(fresh, s.pages + 1);   // more than there are: the sum stays within 32 bits (view() bounds the pages)
   int total;
   const int at = block_scan(cow + fresh, &total, warp_sums);
   give[i] = make_int4(seq, held, at + cow, fresh);
@@ -493,7 +494,7 @@ int view(const rb_kv_pages* a, PagesDev* s) {
   if (row % 16 != 0 || !aligned16(a->store)) return RB_ERR_UNSUPPORTED;
   // a page's pieces, a sequence's tokens and a layer's lists are counted in 32 bits
   if (row * a->page_size * a->kv_heads > (INT64_C(1) << 30) || a->page_size * static_cast<int64_t>(a->max_pages) > (INT64_C(1) << 30) ||
-      a->layers > 16384)
+      a->layers > 16384 || a->pages > (1 << 20))
     return RB_ERR_CAPACITY;
   *s = PagesDev{static_cast<uint8_t*>(a->store), a->layers, a->pages, a->kv_heads, a->page_size, static_cast<int>(row),
                 a->max_seqs, a->max_pages, a->table, a->lengths, a->held, a->refs, a->status};

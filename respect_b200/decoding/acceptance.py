@@ -65,6 +65,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, off
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     M, dev = x.shape[0], x.device
+    if M > 1 and x.stride(0) < V:
+        x = x.contiguous()                   # rows that overlap, as of an expanded tensor
     if top:
         lp, ent, tlp = torch.empty((2 + top) * M, dtype=torch.float32, device=dev).split_with_sizes((M, M, top * M))
         tlp, ids = tlp.view(*lead, top), torch.empty((*lead, top), dtype=torch.int64, device=dev)

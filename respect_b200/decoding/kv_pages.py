@@ -175,9 +175,11 @@ class PagedKVCache:
                                  device=self.device).reshape(len(paths), wide)
         if paths.dtype != torch.int32 or paths.device != self.device or paths.dim() != 2 or paths.shape[0] != s.numel():
             raise ValueError(f"paths must be lists or an int32 tensor [{s.numel()}, width] on {self.device}")
-        paths = paths if paths.stride(-1) == 1 or paths.shape[1] < 2 else paths.contiguous()
-        self._call("rb_kv_pages_compact", s.data_ptr(), paths.data_ptr(), max(paths.stride(0), paths.shape[1]),
-                   paths.shape[1], c.data_ptr(), s.numel(), self._ws.data_ptr(), self._ws_bytes)
+        width = paths.shape[1]
+        if (paths.stride(1) != 1 and width > 1) or paths.stride(0) < width:
+            paths = paths.contiguous()       # rows that overlap, as of an expanded list
+        self._call("rb_kv_pages_compact", s.data_ptr(), paths.data_ptr(), max(paths.stride(0), width), width,
+                   c.data_ptr(), s.numel(), self._ws.data_ptr(), self._ws_bytes)
 
     def truncate(self, seqs, lengths) -> None:
         """Keep lengths[i] tokens of seqs[i]; its other pages, reserved ones too, are given back."""

@@ -79,12 +79,16 @@ def fused_attn_hyb(q, kp, vp, kn, vn, msk, sm_scale=None,
 
 
 def _laid_out(t: torch.Tensor) -> bool:
-    """Unit inner stride, everything else in whole 16-byte pieces."""
+    """Unit inner stride, everything else in whole 16-byte pieces and no dimension repeated in place."""
     *outer, inner = t.stride()
     odd = t.data_ptr() // t.element_size()
     for x in outer:
         odd |= x                     # any low bit set shows
-    return inner == 1 and odd % (16 // t.element_size()) == 0
+    return inner == 1 and odd % (16 // t.element_size()) == 0 and not (0 in outer and _repeats(t))
+
+
+def _repeats(t: torch.Tensor) -> bool:
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
 
 
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
@@ -105,7 +109,9 @@ def _out(out: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
 def _int32(t: torch.Tensor, name: str, dims: int, like: torch.Tensor) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != like.get_device() or t.dim() != dims:
         raise TypeError(f"{name} must be an int32 tensor of {dims} dimension(s) on {like.device}")
-    return t if t.stride(-1) == 1 or t.shape[-1] < 2 else t.contiguous()
+    if (t.stride(-1) != 1 and t.shape[-1] > 1) or (dims == 2 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()               # rows that overlap, as of an expanded table
+    return t
 
 
 def _check_heads(dtype: torch.dtype, heads: int, heads_kv: int, dim: int, dim_kv: int) -> None:
@@ -190,7 +196,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, sm_scale=None, seqs=Non
     dtype = _lib.dtype_code(q.dtype)
     a = _lib.pack_paged_args(dtype, B, H, HK, D, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], sk[2],
                              v.data_ptr(), sv[0], sv[1], sv[2], pages, page_size, table.data_ptr(),
-                             max(table.stride(0), width), width, rows, lengths.data_ptr(),
+                             table.stride(0) if rows > 1 else width, width, rows, lengths.data_ptr(),
                              0 if seqs is None else seqs.data_ptr(), ahead, bound, y.data_ptr(), so[0], so[1],
                              D ** -0.5 if sm_scale is None else sm_scale)
     nbytes = _paged_bytes(dtype, B, H, HK, page_size, width, bound)

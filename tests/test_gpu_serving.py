@@ -284,6 +284,54 @@ def test_captured_and_on_another_stream():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_expanded_and_turned_inputs():
+    """Inputs whose rows repeat in place or lie the other way round are read as what they are."""
+    from respect_b200.decoding.acceptance import token_logprobs
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    from respect_b200.kernels import paged_attention, prompt_attention
+    g = gen(40)
+    for dtype in (BF, F32):
+        q, k, v, table, seqs = paged_inputs(41, [70], 8, 2, 16, dtype)
+        q3 = randn(g, 3, 8, 128, dtype=dtype)
+        want, tol = paged_reference(q3, seqs * 3)
+        close(paged_attention(q3, k, v, table.expand(3, -1), i32([70]).expand(3)), want, tol)
+        close(paged_attention(q3, k, v, table.t().contiguous().t().expand(3, -1), i32([70, 70, 70])), want, tol)
+        kv1 = k[:, :1].expand(-1, 2, -1, -1)             # one head read as two
+        close(paged_attention(q3, kv1, kv1, table.expand(3, -1), i32([70] * 3)),
+              *paged_reference(q3, [(seqs[0][0][:, :1].expand(-1, 2, -1),) * 2] * 3))
+        pq, pk, pv, cu = prompt_inputs(42, [50, 33], 8, 2, dtype)
+        one = pk[:, :1].expand(-1, 2, -1)
+        close(prompt_attention(pq, one, one, i32(cu)), *prompt_reference(pq, one, one, cu))
+        turned = pq.transpose(0, 1).contiguous().transpose(0, 1)
+        assert torch.equal(prompt_attention(turned, pk, pv, i32(cu)), prompt_attention(pq, pk, pv, i32(cu)))
+        odd = randn(g, 83, 8, 129, dtype=dtype)[:, :, 1:]   # rows off the 16-byte grid
+        close(prompt_attention(odd, pk, pv, i32(cu)), *prompt_reference(odd, pk, pv, cu))
+    x = randn(g, 1, 9000).expand(4, -1)
+    tok = torch.tensor([3, 3, 5, 5], device=DEV)
+    a = token_logprobs(x, tok, 5)
+    b = token_logprobs(x.contiguous(), tok, 5)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+    cache = PagedKVCache(1, 1, 16, 4, 3, dtype=F32)
+    cache.reserve([0, 1, 2], [6, 6, 6])
+    cache.write(*token_kv(cache, list(range(18))), [0, 1, 2], [0, 6, 12, 18])
+    cache.compact([0, 1, 2], i32([[1, 4]]).expand(3, -1), i32([2]).expand(3))
+    cache.check()
+    assert cache.lengths.tolist() == [2, 2, 2] and cache.held.tolist() == [1, 1, 1]
+    for s, want in enumerate(([1, 4], [7, 10], [13, 16])):
+        k, _ = token_kv(cache, want)
+        assert torch.equal(cache.store[0, 0, cache.table[s, 0], 0, :2], k[0, :, 0])
+
+
+def test_reserve_of_more_than_32_bits_can_count():
+    """Many sequences asking for everything: refused, nothing changed."""
+    from respect_b200.decoding.kv_pages import PagedCacheError, PagedKVCache
+    cache = PagedKVCache(1, 1, 4, 1, 1000, max_pages=3_000_000, head_dim=8)
+    cache.reserve(list(range(1000)), [3_000_000] * 1000)
+    with pytest.raises(PagedCacheError, match="free pages"):
+        cache.check()
+    assert not bool(cache.refs.any()) and not bool(cache.held.any())
+
+
 # ---------------------------------------------------------------- page operations
 def token_kv(cache, tokens):
     """K / V [layers, n, heads, D] that encode token numbers: distinct for layer, side and head."""

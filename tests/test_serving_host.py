@@ -68,7 +68,8 @@ def test_page_operations_refuse():
     p = 0x700000
     for change, status in ((dict(store=None), INVALID), (dict(status=None), INVALID), (dict(pages=0), INVALID),
                            (dict(page_size=0), INVALID), (dict(elem_bytes=1), UNSUPPORTED), (dict(head_dim=3), UNSUPPORTED),
-                           (dict(store=0x100008), UNSUPPORTED), (dict(max_pages=1 << 28), CAPACITY)):
+                           (dict(store=0x100008), UNSUPPORTED), (dict(max_pages=1 << 28), CAPACITY),
+                           (dict(pages=(1 << 20) + 1), CAPACITY), (dict(layers=20000), CAPACITY)):
         c = ctypes.byref(pages_args(**change))
         assert lib.rb_kv_pages_workspace(c) == 0
         assert lib.rb_kv_pages_commit(c, p, p, 1, None) == status
