@@ -4,7 +4,8 @@ Operators mirror the reference's modules: ``respect_b200.kernels``
 (fused_attn_hyb, linear, rmsnorm, dispatch, patch), ``respect_b200.system.fused``
 (rope, silu_mul), ``respect_b200.decoding`` (verify_trie, FixedKVBuffer, compact,
 greedy_token, walk, the native VerifyEngine) and ``respect_b200.candidates``
-(build_trie, trie_ancestry). All compute runs in librespect_b200.so; there is
+(build_trie, trie_ancestry). Beside them stand prompt_attention and paged_attention
+(``kernels``), PagedKVCache and token_logprobs (``decoding``). All compute runs in librespect_b200.so; there is
 no fallback path.
 """
 __version__ = "0.1.0"

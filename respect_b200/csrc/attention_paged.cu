@@ -15,6 +15,10 @@
 // enters as two bf16 parts (hi + lo), so a weight is good to 2^-16 and the result is
 // rounded once, at the end. fp32: three tf32 products per term, each step from zero and
 // added in fp32. Where pages hold whole tiles, a tile arrives as TMA boxes, else row by row.
+//
+// Measured (both launches, one B200): 64 bf16 sequences of 512 to 12,000 tokens, 32 / 8 heads,
+// 286 us = 5.5 TB/s (with heads as rows and blocks of four warps 335); 256 of 1,024 tokens 5.1
+// TB/s; one of 120,000 4.9 TB/s; one of 4,133, 28 / 4 heads, 14 us, of which most is latency.
 #include <type_traits>
 
 #include "common.cuh"
