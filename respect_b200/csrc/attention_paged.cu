@@ -117,6 +117,7 @@ __device__ __forceinline__ bool item_of(const Dev& p, Item* it) {
   it->k1 = min(static_cast<int64_t>(it->len), it->k0 + static_cast<int64_t>(p.per_warp) * it->chunk);
   return true;
 }
+
 // Where a chunk's result goes: accumulators [B, H, splits, kD], then (max, sum) [B, H, splits].
 __device__ __forceinline__ float* acc_at(const Dev& p, float* part, const Item& it, int r, int c) {
   return part + ((static_cast<int64_t>(it.b) * p.H + it.h0 + r) * p.splits + c) * kD;

@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   if (warp >= kProducerWarp) {   // one setmaxnreg for the whole warpgroup
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kProducerWarp) {
-      uint32_t ring = 0;   // K / V tiles loaded so far
+      uint32_t ring = 0, q_loads = 0;   // K / V tiles, Q pairs loaded so far
       bool ok = true;
       for (int i = 0; ok && next_item(i); ++i) {
         if (lane == 0) {
@@ -536,6 +536,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           if (ok) {
             const int tiles = it.n[1] > 0 ? 2 : 1;
             mbar_arrive_expect_tx(bar(Q_FULL), tiles * 2 * TP * G * 128);
+            ++q_loads;
             for (int t = 0; t < tiles; ++t)
               for (int h = 0; h < 2; ++h)
                 tma_load_4d(sQ + t * kTile + h * kHalf, &tq, bar(Q_FULL), h * 64, 0, it.kvh, it.s0 + it.tok0 + t * TP);
@@ -553,6 +554,10 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      if (!ok && lane == 0) {   // an error flag is up: see the copies in flight out
+        if (q_loads > 0) mbar_wait(bar(Q_FULL), (q_loads - 1) & 1, 0x31d);
+        for (uint32_t x = ring > kRing ? ring - kRing : 0; x < ring; ++x) mbar_wait(bar(KV_FULL + x % kRing), (x / kRing) & 1, 0x31d);
       }
     } else if (warp == kMmaWarp) {
       // The whole warp keeps the books, one lane issues: its loop is nothing but MMAs with

@@ -11,7 +11,7 @@
 // changes nothing.
 //
 // Measured (28 layers, 4 kv heads of 128, bf16, pages of 16): 1,024 drafted tokens of four
-// sequences truncated, reserved, written (59 MB in, 59 MB out) and compacted 38 us; 16
+// sequences truncated, reserved, written (59 MB in, 59 MB out) and compacted 36 us; 16
 // samples forked off two prompts, their last pages copied, one token each, 19 us.
 #include <algorithm>
 
@@ -254,29 +254,39 @@ __global__ void __launch_bounds__(32 * kWriteWarps)
   const int64_t head = static_cast<int64_t>(s.page_size) * vecs;
   const int64_t side = static_cast<int64_t>(s.pages) * s.kv_heads * head;
   uint4* dst0 = reinterpret_cast<uint4*>(s.store) + static_cast<int64_t>(page) * s.kv_heads * head + (pos % s.page_size) * vecs;
-  const int end = min(layers, (static_cast<int>(blockIdx.y) + 1) * each);
-  for (int layer = blockIdx.y * each; layer < end; ++layer) {
-    uint4* dst = dst0 + static_cast<int64_t>(layer0 + layer) * 2 * side;
-    const uint8_t* ks = k.p + layer * k.s_layer + t * k.s_token;
-    const uint8_t* vs = v.p + layer * v.s_layer + t * v.s_token;
-    for (int x0 = lane; x0 < per; x0 += 128) {   // up to eight loads before their stores
-      uint4 a[4], b[4];
+  const int begin = blockIdx.y * each, end = min(layers, begin + each);
+  const uint8_t* kt = k.p + t * k.s_token;
+  const uint8_t* vt = v.p + t * v.s_token;
+  for (int x0 = lane; x0 < per; x0 += 64) {   // two pieces a lane, four layers: up to sixteen loads before their stores
+    const int h0 = x0 / vecs, c0 = x0 % vecs, x1 = x0 + 32, h1 = x1 / vecs, c1 = x1 % vecs;
+    const bool two = x1 < per;
+    const int64_t d0 = h0 * head + c0, d1 = h1 * head + c1;
+    const int64_t k0 = h0 * k.s_head + c0 * 16, k1 = h1 * k.s_head + c1 * 16, v0 = h0 * v.s_head + c0 * 16, v1 = h1 * v.s_head + c1 * 16;
+    for (int l0 = begin; l0 < end; l0 += 4) {
+      uint4 a[4][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = x0 + e * 32, h = x / vecs, c = x % vecs;
-        if (x < per) {
-          a[e] = __ldcs(reinterpret_cast<const uint4*>(ks + h * k.s_head + c * 16));
-          b[e] = __ldcs(reinterpret_cast<const uint4*>(vs + h * v.s_head + c * 16));
+      for (int e = 0; e < 4; ++e)
+        if (l0 + e < end) {
+          const uint8_t* ks = kt + (l0 + e) * k.s_layer;
+          const uint8_t* vs = vt + (l0 + e) * v.s_layer;
+          a[e][0] = __ldcs(reinterpret_cast<const uint4*>(ks + k0));
+          a[e][1] = __ldcs(reinterpret_cast<const uint4*>(vs + v0));
+          if (two) {
+            a[e][2] = __ldcs(reinterpret_cast<const uint4*>(ks + k1));
+            a[e][3] = __ldcs(reinterpret_cast<const uint4*>(vs + v1));
+          }
         }
-      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = x0 + e * 32, h = x / vecs, c = x % vecs;
-        if (x < per) {
-          dst[h * head + c] = a[e];
-          dst[side + h * head + c] = b[e];
+      for (int e = 0; e < 4; ++e)
+        if (l0 + e < end) {
+          uint4* dst = dst0 + static_cast<int64_t>(layer0 + l0 + e) * 2 * side;
+          dst[d0] = a[e][0];
+          dst[side + d0] = a[e][1];
+          if (two) {
+            dst[d1] = a[e][2];
+            dst[side + d1] = a[e][3];
+          }
         }
-      }
     }
   }
 }
@@ -546,8 +556,8 @@ int kv_pages_write(const rb_kv_pages* a, const rb_kv_tokens* x, const int32_t* s
   if (!aligned16(x->k) || !aligned16(x->v)) return RB_ERR_UNSUPPORTED;
   const WriteSrc k{static_cast<const uint8_t*>(x->k), x->skl * es, x->skt * es, x->skh * es};
   const WriteSrc v{static_cast<const uint8_t*>(x->v), x->svl * es, x->svt * es, x->svh * es};
-  // about 32 warps an SM before a warp takes a second layer
-  const int64_t work = static_cast<int64_t>(x->tokens) * x->layers / (device_sm_count() * 32);
+  // about 16 warps an SM before a warp takes more layers; four at a time are in flight
+  const int64_t work = static_cast<int64_t>(x->tokens) * x->layers / (device_sm_count() * 16);
   const int each = static_cast<int>(work < 1 ? 1 : work > 8 ? 8 : work);
   return launch_k(write_tokens, dim3(ceil_div(x->tokens, kWriteWarps), ceil_div(x->layers, each)), dim3(32 * kWriteWarps), 0,
                   st, true, s, k, v, seqs, offsets, n, x->tokens, x->layer0, x->layers, each);
