@@ -338,29 +338,32 @@ __global__ void __launch_bounds__(kThreads, TOP ? (sizeof(T) == 4 ? 5 : 4) : 6)
 }
 
 // The row's sums in order, by one warp, and the chunks' best entries: a block per row with
-// alternatives (its warps share the lists), a warp per row without.
-constexpr int kJoinWarps = 4;
+// alternatives (warp 0 has the sums, the others share the lists meanwhile), a warp per row
+// without.
+template <bool TOP>
+constexpr int kJoinWarps = TOP ? 9 : 4;
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(32 * kJoinWarps)
+__global__ void __launch_bounds__(32 * kJoinWarps<TOP>)
     join_kernel(const T* __restrict__ logits, int64_t ld, int M, int V, const int64_t* __restrict__ tokens, int off,
                 int size, int top, int chunks, const Stat* __restrict__ stats, const uint64_t* __restrict__ best,
                 float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ top_lp,
                 int64_t* __restrict__ top_ids) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = TOP ? blockIdx.x : blockIdx.x * kJoinWarps + warp;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = TOP ? blockIdx.x : blockIdx.x * kJoinWarps<TOP> + warp;
   if (row >= M) return;
-  uint64_t k = 0;
+  __shared__ uint64_t lists[TOP ? kJoinWarps<TOP> - 1 : 1][32];
   if constexpr (TOP) {
-    __shared__ uint64_t lists[kJoinWarps][32];
-    const uint64_t* b = best + static_cast<int64_t>(row) * chunks * top;
+    if (warp > 0) {
+      const uint64_t* b = best + static_cast<int64_t>(row) * chunks * top;
+      uint64_t k = 0;
 #pragma unroll 4
-    for (int c = warp; c < chunks; c += kJoinWarps) k = warp_merge_desc(k, lane < top ? b[static_cast<int64_t>(c) * top + lane] : uint64_t(0));
-    lists[warp][lane] = k;
-    __syncthreads();
-    if (warp > 0) return;
-#pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) k = warp_merge_desc(k, lists[w][lane]);
+      for (int c = warp - 1; c < chunks; c += kJoinWarps<TOP> - 1)
+        k = warp_merge_desc(k, lane < top ? b[static_cast<int64_t>(c) * top + lane] : uint64_t(0));
+      lists[warp - 1][lane] = k;
+      __syncthreads();
+      return;
+    }
   }
   const int64_t parts = static_cast<int64_t>(chunks) * kWarps;
   const float4* st = reinterpret_cast<const float4*>(stats + row * parts);
@@ -399,6 +402,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     entropy[row] = bad ? nan_f : logs - t / s;
   }
   if constexpr (TOP) {
+    __syncthreads();
+    uint64_t k = lists[0][lane];
+#pragma unroll
+    for (int w = 1; w < kJoinWarps<TOP> - 1; ++w) k = warp_merge_desc(k, lists[w][lane]);
     if (lane < top) {
       top_lp[static_cast<int64_t>(row) * top + lane] = bad ? nan_f : value_of(k) - top_m - logs;
       top_ids[static_cast<int64_t>(row) * top + lane] = index_of(k);
@@ -416,13 +423,14 @@ int run(const void* logits, int64_t ld, int M, int V, const int64_t* tokens, int
   Stat* stats = static_cast<Stat*>(ws);
   uint64_t* best = reinterpret_cast<uint64_t*>(stats + static_cast<int64_t>(M) * chunks * kWarps);
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(M) * chunks));
-  auto go = [&](auto chunk, auto join, int rows_per_block) {
+  auto go = [&](auto chunk, auto join, int rows_per_block, int threads) {
     const int r = launch_k(chunk, grid, dim3(kThreads), 0, st, true, x, ld, V, off, size, top, chunks, stats, best);
     if (r != RB_OK) return r;
-    return launch_k(join, dim3((M + rows_per_block - 1) / rows_per_block), dim3(32 * kJoinWarps), 0, st, true, x, ld, M, V, tokens,
+    return launch_k(join, dim3((M + rows_per_block - 1) / rows_per_block), dim3(threads), 0, st, true, x, ld, M, V, tokens,
                     off, size, top, chunks, stats, best, logprob, entropy, top_lp, top_ids);
   };
-  return top > 0 ? go(chunk_kernel<T, true>, join_kernel<T, true>, 1) : go(chunk_kernel<T, false>, join_kernel<T, false>, kJoinWarps);
+  return top > 0 ? go(chunk_kernel<T, true>, join_kernel<T, true>, 1, 32 * kJoinWarps<true>)
+                 : go(chunk_kernel<T, false>, join_kernel<T, false>, kJoinWarps<false>, 32 * kJoinWarps<false>);
 }
 
 }  // namespace lp
