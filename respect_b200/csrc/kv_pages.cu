@@ -317,10 +317,11 @@ __global__ void __launch_bounds__(kPlanThreads)
 
 // ---------------------------------------------------------------- fork
 // Plan: every pair is valid (sources exist, targets are distinct, empty and no
-// source of the call); ok[0] tells the pairs' blocks.
+// source of the call); ok[0] tells the pairs' blocks, unless (`share`) the plan's block,
+// a warp per pair, shares the pages itself.
 __global__ void __launch_bounds__(kPlanThreads)
     fork_plan(const PagesDev s, const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int n,
-              int32_t* __restrict__ ok) {
+              int32_t* __restrict__ ok, bool share) {
   __shared__ int set[kHash];
   pdl_wait();
   pdl_trigger();
@@ -335,6 +336,19 @@ __global__ void __launch_bounds__(kPlanThreads)
   if (i == 0) {
     ok[0] = good;
     if (!good) refuse(s, RB_PAGES_BAD_SEQUENCE);
+  }
+  if (!good || !share) return;
+  for (int e = i >> 5; e < n; e += kPlanThreads / 32) {
+    const int a = src[e], d = dst[e], len = s.lengths[a], pages = ceil_div(len, s.page_size);
+    for (int x = i & 31; x < pages; x += 32) {
+      const int p = s.table[static_cast<int64_t>(a) * s.max_pages + x];
+      s.table[static_cast<int64_t>(d) * s.max_pages + x] = p;
+      if (p >= 0 && p < s.pages) atomicAdd(&s.refs[p], 1);
+    }
+    if ((i & 31) == 0) {
+      s.lengths[d] = len;
+      s.held[d] = pages;
+    }
   }
 }
 // Block (x, pair): the pages that hold the source's tokens become the target's too.
@@ -581,8 +595,10 @@ int kv_pages_fork(const rb_kv_pages* a, const int32_t* src, const int32_t* dst, 
   if (!src || !dst) return RB_ERR_INVALID_ARG;
   if (!ws || bytes < kv_pages_workspace(a)) return RB_ERR_WORKSPACE;
   int32_t* ok = static_cast<int32_t*>(ws);
-  r = launch_k(fork_plan, dim3(1), dim3(kPlanThreads), 0, st, true, s, src, dst, n, ok);
-  if (r != RB_OK) return r;
+  // up to 16 passes of the plan's block over the tables cost less than a second launch
+  const bool share = static_cast<int64_t>(n) * s.max_pages <= 16 * kPlanThreads;
+  r = launch_k(fork_plan, dim3(1), dim3(kPlanThreads), 0, st, true, s, src, dst, n, ok, share);
+  if (r != RB_OK || share) return r;
   return launch_k(fork_share, dim3(std::min(8, ceil_div(s.max_pages, 256)), n), dim3(256), 0, st, true, s, src, dst,
                   ok);
 }

@@ -491,6 +491,25 @@ def test_page_operations_refuse_and_change_nothing():
     cache.check()
 
 
+def test_forks_of_long_tables():
+    """Tables too large for the plan's own block: the same result through a block per pair."""
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    cache = PagedKVCache(1, 1, 3000, 2, 8, max_pages=5000, dtype=F32)
+    model = Pages(3000, 2, 8, 5000)
+    cache.reserve([1, 6], [4001, 333])
+    cache.commit([1, 6], [4001, 333])
+    cache.fork([1, 6, 1, 6], [0, 7, 3, 2])
+    cache.check()
+    model.reserve([1, 6], [4001, 333])
+    model.lengths[1], model.lengths[6] = 4001, 333
+    for a, d in ((1, 0), (6, 7), (1, 3), (6, 2)):
+        model.fork(a, d)
+    assert cache.lengths.tolist() == model.lengths and cache.refs.tolist() == model.refs
+    assert cache.held.tolist() == [len(r) for r in model.rows]
+    for i, r in enumerate(cache.table.tolist()):
+        assert [x for x in r if x >= 0] == model.rows[i]
+
+
 def test_page_operations_captured():
     """A decoding round captured once and replayed: each replay is the next token."""
     from respect_b200.decoding.kv_pages import PagedKVCache
