@@ -27,6 +27,11 @@ constexpr int kHash = 2 * RB_PAGES_MAX_LIST;   // open addressing at load <= 1/2
 
 __device__ __forceinline__ void refuse(const PagesDev& s, int code) { atomicCAS(s.status, 0, code); }
 
+// A sequence's pages and tokens, within what its row of the table can hold whatever the
+// caller's state says.
+__device__ __forceinline__ int held_of(const PagesDev& s, int seq) { return min(max(s.held[seq], 0), s.max_pages); }
+__device__ __forceinline__ int length_of(const PagesDev& s, int seq) { return min(max(s.lengths[seq], 0), s.max_pages * s.page_size); }
+
 // Inserts v into an open-addressed set of kHash words (-1 = empty); false if it was there.
 __device__ __forceinline__ bool set_insert(int* set, int v) {
   int at = (static_cast<uint32_t>(v) * 2654435761u) % kHash;
@@ -111,8 +116,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   bool bad = false;
   if (i < n) {
     seq = seqs[i];
-    len = s.lengths[seq];
-    held = s.held[seq];
+    len = length_of(s, seq);
+    held = held_of(s, seq);
     count = counts[i];
     bad = count < 0 || count > static_cast<int64_t>(s.max_pages) * ps - len;
     if (!bad && count > 0 && len % ps != 0) {
@@ -239,9 +244,9 @@ __global__ void __launch_bounds__(32 * kWriteWarps)
     if (lane == 0) refuse(s, RB_PAGES_BAD_SEQUENCE);
     return;
   }
-  const int64_t pos = static_cast<int64_t>(s.lengths[seq]) + j;
+  const int64_t pos = static_cast<int64_t>(length_of(s, seq)) + j;
   const int64_t idx = pos / s.page_size;
-  if (idx >= s.held[seq]) {
+  if (idx >= held_of(s, seq)) {
     if (lane == 0) refuse(s, RB_PAGES_BAD_COUNT);
     return;
   }
@@ -305,8 +310,8 @@ __global__ void __launch_bounds__(kPlanThreads)
   int64_t len = 0;
   bool bad = false;
   if (i < n) {
-    len = static_cast<int64_t>(s.lengths[seqs[i]]) + counts[i];
-    bad = counts[i] < 0 || len > static_cast<int64_t>(s.held[seqs[i]]) * s.page_size;
+    len = static_cast<int64_t>(length_of(s, seqs[i])) + counts[i];
+    bad = counts[i] < 0 || len > static_cast<int64_t>(held_of(s, seqs[i])) * s.page_size;
   }
   if (__syncthreads_or(bad)) {
     if (i == 0) refuse(s, RB_PAGES_BAD_COUNT);
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   bool bad = false;
   if (good && i < n) {
     const int a = src[i];
-    bad = a < 0 || a >= s.max_seqs || set_has(set, a) || s.held[dst[i]] != 0 || s.lengths[dst[i]] != 0;
+    bad = a < 0 || a >= s.max_seqs || set_has(set, a) || held_of(s, dst[i]) != 0 || length_of(s, dst[i]) != 0;
   }
   good = !__syncthreads_or(bad) && good;
   if (i == 0) {
@@ -339,7 +344,7 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   if (!good || !share) return;
   for (int e = i >> 5; e < n; e += kPlanThreads / 32) {
-    const int a = src[e], d = dst[e], len = s.lengths[a], pages = ceil_div(len, s.page_size);
+    const int a = src[e], d = dst[e], len = length_of(s, a), pages = ceil_div(len, s.page_size);
     for (int x = i & 31; x < pages; x += 32) {
       const int p = s.table[static_cast<int64_t>(a) * s.max_pages + x];
       s.table[static_cast<int64_t>(d) * s.max_pages + x] = p;
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(256)
   pdl_trigger();
   if (!ok[0]) return;
   const int a = src[blockIdx.y], d = dst[blockIdx.y];
-  const int len = s.lengths[a], pages = ceil_div(len, s.page_size);
+  const int len = length_of(s, a), pages = ceil_div(len, s.page_size);
   for (int x = blockIdx.x * blockDim.x + threadIdx.x; x < pages; x += gridDim.x * blockDim.x) {
     const int p = s.table[static_cast<int64_t>(a) * s.max_pages + x];
     s.table[static_cast<int64_t>(d) * s.max_pages + x] = p;
@@ -395,13 +400,13 @@ __global__ void __launch_bounds__(256)
   }
   bool bad = false;
   if (lengths)
-    for (int i = threadIdx.x; i < n; i += blockDim.x) bad |= lengths[i] < 0 || lengths[i] > s.lengths[seqs[i]];
+    for (int i = threadIdx.x; i < n; i += blockDim.x) bad |= lengths[i] < 0 || lengths[i] > length_of(s, seqs[i]);
   if (__syncthreads_or(bad)) {
     if (threadIdx.x == 0) refuse(s, RB_PAGES_BAD_COUNT);
     return;
   }
   const int seq = seqs[blockIdx.x], len = lengths ? lengths[blockIdx.x] : 0;
-  const int keep = ceil_div(len, s.page_size), held = s.held[seq];
+  const int keep = ceil_div(len, s.page_size), held = held_of(s, seq);
   release(s, seq, keep, held);
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -425,8 +430,8 @@ __global__ void __launch_bounds__(256)
     }
     return;
   }
-  const int seq = seqs[blockIdx.x], m = counts[blockIdx.x], len = s.lengths[seq];
-  const int64_t room = static_cast<int64_t>(s.held[seq]) * s.page_size - len;
+  const int seq = seqs[blockIdx.x], m = counts[blockIdx.x], len = length_of(s, seq);
+  const int64_t room = static_cast<int64_t>(held_of(s, seq)) * s.page_size - len;
   const int32_t* path = paths + blockIdx.x * ld;
   bool bad = m < 0 || m > width, shared = false;
   if (!bad)
@@ -464,7 +469,7 @@ __global__ void __launch_bounds__(kMoveThreads)
   pdl_wait();
   pdl_trigger();
   if (refused(flags, n)) return;
-  const int seq = seqs[blockIdx.y], m = counts[blockIdx.y], len = s.lengths[seq];
+  const int seq = seqs[blockIdx.y], m = counts[blockIdx.y], len = length_of(s, seq);
   const int vecs = s.row_bytes / 16;
   const int64_t head = static_cast<int64_t>(s.page_size) * vecs, page = head * s.kv_heads;
   const int64_t x = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x;
@@ -501,8 +506,8 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   pdl_trigger();
   if (refused(flags, n)) return;
-  const int seq = seqs[blockIdx.x], len = s.lengths[seq] + counts[blockIdx.x];
-  const int keep = ceil_div(len, s.page_size), held = s.held[seq];
+  const int seq = seqs[blockIdx.x], len = length_of(s, seq) + counts[blockIdx.x];
+  const int keep = ceil_div(len, s.page_size), held = held_of(s, seq);
   release(s, seq, keep, held);
   __syncthreads();
   if (threadIdx.x == 0) {

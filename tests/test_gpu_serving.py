@@ -491,6 +491,30 @@ def test_page_operations_refuse_and_change_nothing():
     cache.check()
 
 
+def test_counts_beyond_the_table():
+    """A state whose counts name more than a row of the table holds: the next rows stay as they were."""
+    from respect_b200.decoding.kv_pages import PagedCacheError, PagedKVCache
+    cache = PagedKVCache(1, 1, 32, 4, 4, max_pages=4, dtype=F32)
+    cache.reserve([0, 1], [16, 16])
+    cache.commit([0, 1], [16, 16])
+    cache.held[0], cache.lengths[0] = 8, 32
+    cache.reserve([0], [1])                 # its row is full
+    with pytest.raises(PagedCacheError, match="room"):
+        cache.check()
+    cache.fork([0], [2])
+    cache.check()
+    assert cache.lengths[2].item() == 16 and torch.equal(cache.table[2], cache.table[0])
+    cache.free([0])
+    cache.check()
+    assert cache.table[0].tolist() == [-1] * 4 and cache.table[1].tolist() == [4, 5, 6, 7]
+    assert cache.refs.tolist() == [1] * 8 + [0] * 24
+    assert cache.held.tolist() == [0, 4, 4, 0] and cache.lengths.tolist() == [0, 16, 16, 0]
+    cache.held[3], cache.lengths[3] = -2, -9
+    cache.reserve([3], [5])
+    cache.check()
+    assert cache.held[3].item() == 2 and cache.table[3].tolist() == [8, 9, -1, -1]
+
+
 def test_forks_of_long_tables():
     """Tables too large for the plan's own block: the same result through a block per pair."""
     from respect_b200.decoding.kv_pages import PagedKVCache
