@@ -183,11 +183,16 @@ __device__ __noinline__ void redo_row(const Dev& p, const Item& it, float* part,
 constexpr int kQPitch = kD + 4;
 template <typename T, bool kTma>
 struct Ring {
-  static constexpr int kStages = sizeof(T) == 2 ? 3 : 2;   // tiles in a warp's ring: eight bf16 warps an SM, five fp32
+  // Tiles in a warp's ring. fp32 tiles are twice as large and take long to compute: eight warps
+  // an SM with a tile each hide more than five with two (32 sequences of 2,048 tokens, 28 / 4
+  // heads: 91 us against 124; one of 4,133: 15 either way).
+  static constexpr int kStages = sizeof(T) == 2 ? 3 : 1;
   static constexpr int kRow = kD * sizeof(T);
   static constexpr int kSide = kKeys * (kTma ? kRow : kRow + 16), kTile = 2 * kSide;
   // ring, mbarriers, fp32: the tile's weights and the queries (pitches free of bank conflicts)
-  static constexpr int kSmem = 1024 + kStages * kTile + 64 + (sizeof(T) == 4 ? (kKeys * 20 + kRows * kQPitch) * 4 : 0);
+  static constexpr int smem(int nt) {
+    return 1024 + kStages * kTile + 64 + (sizeof(T) == 4 ? (kKeys * (nt == 1 ? 12 : 20) + nt * 8 * kQPitch) * 4 : 0);
+  }
   __device__ __forceinline__ static uint32_t at(uint32_t side, int row, int piece) {
     return kTma ? side + (piece >> 3) * (kKeys * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16) : side + row * (kRow + 16) + piece * 16;
   }
@@ -325,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 8)
 
   constexpr int kPitch = NT == 1 ? 12 : 20;   // fp32 weights, [key][head]: free of bank conflicts
   float* weights = reinterpret_cast<float*>(sm + kStages * kTile + 64);
-  uint32_t* queries = reinterpret_cast<uint32_t*>(weights + kKeys * 20);
+  uint32_t* queries = reinterpret_cast<uint32_t*>(weights + kKeys * kPitch);
   uint32_t there[kStages];                 // which keys there are of tiles t, t + 1, ...
   int page = page_at(0);
 #pragma unroll
@@ -371,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 8)
   int left = per_chunk, chunk = it.c0;
   uint32_t phase = 0;
   for (int t0 = 0; t0 < tiles; t0 += kStages, phase ^= 1) {
-#pragma unroll(sizeof(T) == 2 ? kStages : 1)   // fp32 has code enough as it is
+#pragma unroll
     for (int s = 0; s < kStages; ++s) {
       const int t = t0 + s;
       if (t >= tiles) break;
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[n][e] = odd[n][e] = 0.f;
         const int kr = lane & 15;                                   // ldmatrix rows: keys 0-7, 8-15, then the next 8 dims
-#pragma unroll(sizeof(T) == 2 ? kSteps : 4)
+#pragma unroll
         for (int kk = 0; kk < kSteps; ++kk) {   // ldmatrix moves 8 x 4 fp32 blocks as it moves 8 x 8 bf16 ones
           uint32_t a[4];
           ldsm4(R::at(K, kr, kk * 2 + (lane >> 4)), a);
@@ -442,14 +447,14 @@ __global__ void __launch_bounds__(kThreads, 8)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               *reinterpret_cast<float2*>(weights + (g + h * 8) * kPitch + n * 8 + c * 2) = make_float2(sc[n][2 * h], sc[n][2 * h + 1]);
-            continue;
-          }
+          } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {   // keys g, then g + 8: rows of an 8 x 8 matrix, turned into columns
-            const float x = sc[n][2 * h], y = sc[n][2 * h + 1];
-            const uint32_t u = pack_bf16x2(x, y);
-            hi[n][h] = transpose8(u);
-            lo[n][h] = transpose8(pack_bf16x2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
+            for (int h = 0; h < 2; ++h) {   // keys g, then g + 8: rows of an 8 x 8 matrix, turned into columns
+              const float x = sc[n][2 * h], y = sc[n][2 * h + 1];
+              const uint32_t u = pack_bf16x2(x, y);
+              hi[n][h] = transpose8(u);
+              lo[n][h] = transpose8(pack_bf16x2(x - __uint_as_float(u << 16), y - __uint_as_float(u & 0xFFFF0000u)));
+            }
           }
         }
         if (!__all_sync(0xffffffffu, same)) {
@@ -680,7 +685,7 @@ int paged_launch(const rb_paged_args* a, void* ws, size_t ws_bytes, cudaStream_t
   auto both = [&](auto zero, auto nt) {
     using T = decltype(zero);
     constexpr int NT = decltype(nt)::value;
-    return tma ? go(paged_kernel<T, NT, true>, Ring<T, true>::kSmem) : go(paged_kernel<T, NT, false>, Ring<T, false>::kSmem);
+    return tma ? go(paged_kernel<T, NT, true>, Ring<T, true>::smem(NT)) : go(paged_kernel<T, NT, false>, Ring<T, false>::smem(NT));
   };
   const std::integral_constant<int, 1> nt1{};
   const std::integral_constant<int, 2> nt2{};
