@@ -150,7 +150,8 @@ RB_API int rb_prompt_attn(const rb_prompt_args* a, void* stream);
  * r = seqs[b] (NULL: r = b), cut to [0, min(width * page_size, max_length)]
  * (max_length 0: no further bound). A length of 0, a row outside [0, rows) and
  * a sequence none of whose pages exist give zeros; entries outside [0, pages)
- * name no page and their tokens are left out. The cache is cut into chunks at
+ * name no page and their tokens are left out; scores that are all -inf give NaN,
+ * as in rb_prompt_attn. The cache is cut into chunks at
  * absolute positions whose size depends on the sequence's length alone, joined
  * in order, so a row's bits do not depend on the batch. Unit inner strides, other
  * strides and bases in whole 16-byte pieces, D = 128. */

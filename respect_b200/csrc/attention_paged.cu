@@ -92,6 +92,10 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
+// The weights' sum of a chunk none of whose tokens has a page: tells it from one whose scores are
+// all -inf, whose sum is 0 (and whose sequence, if nothing else is in it, has no value: 0 / 0).
+constexpr float kNothing = -1.f;
+
 // What a warp works on: consecutive chunks of one sequence and kv head.
 struct Item {
   int b, kvh, h0, nh;        // batch entry, kv head, first query head and how many
@@ -374,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 8)
   };
   reset();
   int left = per_chunk, chunk = it.c0;
+  bool some = false;                       // a token of the chunk has a page; the same in every lane
   uint32_t phase = 0;
   for (int t0 = 0; t0 < tiles; t0 += kStages, phase ^= 1) {
 #pragma unroll
@@ -397,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 8)
             asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(R::at(V, x / kPieces, x % kPieces)), "r"(0) : "memory");
       }
       __syncwarp();
+      some |= live != 0u;
       if (live) {   // the same in every lane
         float sc[NT][4], odd[NT][4];   // bf16: the odd steps apart, which halves the chain of dependent products
 #pragma unroll
@@ -513,7 +519,6 @@ __global__ void __launch_bounds__(kThreads, 8)
             bool nan = false;
             if (r < it.nh) {
               if (it.chunks == 1) {
-                const bool some = sum > 0.f || sum != sum;   // no token at all: zeros
                 T* dst = out_at<T>(p, it, r) + g;
 #pragma unroll
                 for (int d = 0; d < kD / 16; ++d)
@@ -533,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 8)
                     nan |= o[d][n][h * 2 + e] != o[d][n][h * 2 + e];
                     dst[d * 16 + h * 8] = o[d][n][h * 2 + e];
                   }
-                if (g == 0) *ml_at(p, part, it, r, chunk) = make_float2(m[n][e], sum);
+                if (g == 0) *ml_at(p, part, it, r, chunk) = make_float2(m[n][e], some ? sum : kNothing);
               }
             }
             const unsigned again = __ballot_sync(0xffffffffu, nan);
@@ -544,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 8)
           }
         reset();
         left = per_chunk;
+        some = false;
         ++chunk;
       }
 #pragma unroll
@@ -559,6 +565,7 @@ template <typename T>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks(const Dev p, const float* __restrict__ part) {
   __shared__ float4 accs[kJoinWarps][32];
   __shared__ float sums[kJoinWarps];
+  __shared__ bool any[kJoinWarps];
   pdl_wait();
   pdl_trigger();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -574,11 +581,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks(const Dev p, cons
   const float ref = m == -INFINITY ? 0.f : m;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
+  bool some = false;
 #pragma unroll 4
   for (int c = warp; c < n; c += kJoinWarps) {
     const float2 x = ml[c];
     const float4 v = acc[c * (kD / 4)];
-    const float f = fast_exp2(x.x - ref);   // 0 for a chunk none of whose tokens has a page
+    const float f = fast_exp2(x.x - ref);   // 0 for a chunk with nothing in it
+    some |= x.y != kNothing;
     a.x = fmaf(f, v.x, a.x);
     a.y = fmaf(f, v.y, a.y);
     a.z = fmaf(f, v.z, a.z);
@@ -586,7 +595,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks(const Dev p, cons
     l = fmaf(f, x.y, l);
   }
   accs[warp][lane] = a;
-  if (lane == 0) sums[warp] = l;
+  if (lane == 0) {
+    sums[warp] = l;
+    any[warp] = some;
+  }
   __syncthreads();
   if (warp > 0) return;
 #pragma unroll
@@ -597,8 +609,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_chunks(const Dev p, cons
     a.z += v.z;
     a.w += v.w;
     l += sums[w];
+    some |= any[w];
   }
-  const bool some = l > 0.f || l != l;
   const float4 y = some ? make_float4(a.x / l, a.y / l, a.z / l, a.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
   const int64_t at = b * p.sob + h * p.soh + lane * 4;
   if (sizeof(T) == 4) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = y;

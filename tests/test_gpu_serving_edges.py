@@ -1,0 +1,39 @@
+"""The serving operators where values are not finite, where a call is refused half way through a decoding
+round, and at sizes that reach the paths of large launches. Tolerances: tests/serving_reference.py."""
+import pytest
+import torch
+
+from tests.serving_reference import close
+from tests.test_gpu_serving import BF, F32, i32, paged_inputs, paged_reference
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+# ---------------------------------------------------------------- scores of minus infinity
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_every_score_minus_infinity_is_not_an_empty_row(dtype):
+    """A softmax over scores that are all -inf has no value, whether one chunk holds them or many; a sequence
+    without a page is zero all the same."""
+    from respect_b200.kernels import paged_attention, prompt_attention
+    lens = [1, 40, 700, 700, 500, 300, 130]
+    q, k, v, table, seqs = paged_inputs(51, lens, 8, 2, 16, dtype)
+    q[..., 0] = q[..., 0].abs() + 1
+    ref, tol = paged_reference(q, seqs)
+    for b, n in enumerate(lens):
+        first = 0 if b != 3 else 350                        # sequence 3: its first half stays as it is
+        if b == 5:
+            continue                                        # as it is throughout
+        for j in range(first, n):
+            k[table[b, j // 16], :, j % 16, 0] = -INF
+    table[4, :5], table[4, 9] = -1, -1                      # pages missing before and among them
+    table[6] = -1
+    ref[[0, 1, 2, 4]] = NAN
+    ref[6] = 0
+    ref[3], tol[3] = (x[0] for x in paged_reference(q[3:4], [(seqs[3][0][:350], seqs[3][1][:350])]))
+    y = paged_attention(q, k, v, table, i32(lens))
+    close(y, ref, tol)
+    kk = seqs[1][0].clone()
+    kk[:, :, 0] = -INF
+    p = prompt_attention(q[1:2].expand(40, -1, -1), kk, seqs[1][1], i32([0, 40]))
+    assert torch.equal(p[39].isnan(), y[1].isnan()) and bool(p.isnan().all())
