@@ -142,7 +142,8 @@ __device__ __forceinline__ void write_empty(const Dev& p, const Item& it) {   //
 
 // Row r of chunk c again, by one warp and key by key. A product in several parts turns an
 // infinity into a NaN (infinity times a second part of zero) that the plain product is
-// not; a row that came out NaN is settled here.
+// not; a row that came out NaN is settled here. A weight that is zero, or that a later
+// maximum makes zero, turns an attended infinity or NaN into a NaN, as in the tiles.
 template <typename T>
 __device__ __noinline__ void redo_row(const Dev& p, const Item& it, float* part, int r, int c) {
   const int lane = threadIdx.x & 31, d = lane * 4;
@@ -167,7 +168,7 @@ __device__ __noinline__ void redo_row(const Dev& p, const Item& it, float* part,
     m = mx;
     l = fmaf(l, a, x);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = a == 0.f ? x * v[e] : fmaf(o[e], a, x * v[e]);
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], a, x * v[e]);
   }
   if (it.chunks == 1) {
 #pragma unroll

@@ -115,7 +115,7 @@ __device__ __noinline__ void redo_row(const Dev& p, int s0, int tok, int h) {
     bool nan = true;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[e] = a == 0.f ? w * v[e] : fmaf(o[e], a, w * v[e]);
+      o[e] = fmaf(o[e], a, w * v[e]);
       nan &= o[e] != o[e];
     }
     if (__all_sync(0xffffffffu, nan || l != l)) break;   // nothing changes any more

@@ -37,3 +37,28 @@ def test_every_score_minus_infinity_is_not_an_empty_row(dtype):
     kk[:, :, 0] = -INF
     p = prompt_attention(q[1:2].expand(40, -1, -1), kk, seqs[1][1], i32([0, 40]))
     assert torch.equal(p[39].isnan(), y[1].isnan()) and bool(p.isnan().all())
+
+
+# ---------------------------------------------------------------- bad values beside a key that takes everything
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n,bad,best", [(40, 3, 30), (40, 30, 3), (300, 5, 20), (300, 20, 5), (300, 5, 290), (300, 290, 5)])
+def test_a_nan_beside_a_dominating_key_stays(dtype, n, bad, best):
+    """An attended NaN shows wherever the key lies that takes all the weight: before it, after it, in the same
+    chunk or tile or in another."""
+    from respect_b200.kernels import paged_attention, prompt_attention
+    q, k, v, table, seqs = paged_inputs(52, [n], 8, 2, 16, dtype)
+    q[..., 0] = 40.0
+    k[table[0, best // 16], :, best % 16, 0] = 40.0         # a score of 1600 / sqrt(128): the others weigh 2^-200
+    v[table[0, bad // 16], 1, bad % 16, 9] = NAN
+    # the plain value of the other entries: V of the dominating key, up to weights of 2^-180
+    ref, tol = paged_reference(q, [(seqs[0][0][best:best + 1], seqs[0][1][best:best + 1])])
+    ref[0, 4:, 9] = NAN
+    close(paged_attention(q, k, v, table, i32([n])), ref, tol)
+    kk, vv = seqs[0][0].clone(), seqs[0][1].clone()
+    kk[best, :, 0], vv[bad, 1, 9] = 40.0, NAN
+    y = prompt_attention(q.expand(n, -1, -1), kk, vv, i32([0, n]))
+    ref, tol = ref.expand(n, -1, -1).clone(), tol * (1 if dtype == F32 else 2)   # bf16 prompts: one part of P, 2^-8 more
+    ref[:bad, 4:, 9] = seqs[0][1][best, 1, 9].double()
+    close(y[max(best, bad):], ref[max(best, bad):], tol.expand(n, -1, -1)[max(best, bad):])
+    if best < bad:
+        close(y[best:bad], ref[best:bad], tol.expand(n, -1, -1)[best:bad])
