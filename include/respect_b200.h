@@ -279,7 +279,8 @@ RB_API int rb_compact_kv(void* const* k_layers, void* const* v_layers, int n_lay
  *             committed before the call are not kept by such a copy.
  *   write     tokens t in [offsets[i], offsets[i + 1]) (NULL: token i) go to
  *             positions lengths[i] + t - offsets[i], inside reserved room.
- *   commit    lengths[i] += counts[i], inside reserved room.
+ *   commit    lengths[i] += counts[i], inside reserved room, on pages that no other
+ *             sequence holds (so before a fork, not after it).
  *   fork      an empty sequence dst[i] takes the tokens of src[i] (pages shared).
  *   compact   kv_buffer.py:93-104 on pages: the written positions lengths[i] +
  *             paths[i, j], j < counts[i] (strictly increasing) move to lengths[i]
@@ -292,7 +293,7 @@ enum rb_pages_status {
   RB_PAGES_BAD_SEQUENCE = 1, /* a sequence that does not exist, is named twice, or a fork's target in use */
   RB_PAGES_NONE_FREE = 2,    /* fewer free pages than the call needs */
   RB_PAGES_BAD_COUNT = 3,    /* a count, length, path or position outside the sequence's room */
-  RB_PAGES_SHARED = 4        /* a write into a page that another sequence holds (reserve again after a fork) */
+  RB_PAGES_SHARED = 4        /* a write or commit into a page that another sequence holds (reserve again after a fork) or that is missing */
 };
 typedef struct rb_kv_pages {
   void* store;

@@ -297,6 +297,10 @@ __global__ void __launch_bounds__(32 * kWriteWarps)
 }
 
 // ---------------------------------------------------------------- commit
+// A sequence takes only what a write could have put there: every position within the pages it
+// holds, on pages that nobody else does. So a round whose reserve or write was refused (the
+// host need not look in between) does not make tokens of what was never written. A warp per entry
+// looks at the pages.
 __global__ void __launch_bounds__(kPlanThreads)
     commit_plan(const PagesDev s, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int n) {
   __shared__ int set[kHash];
@@ -308,13 +312,25 @@ __global__ void __launch_bounds__(kPlanThreads)
   }
   const int i = threadIdx.x;
   int64_t len = 0;
-  bool bad = false;
+  bool bad = false, shared = false;
   if (i < n) {
     len = static_cast<int64_t>(length_of(s, seqs[i])) + counts[i];
     bad = counts[i] < 0 || len > static_cast<int64_t>(held_of(s, seqs[i])) * s.page_size;
   }
   if (__syncthreads_or(bad)) {
     if (i == 0) refuse(s, RB_PAGES_BAD_COUNT);
+    return;
+  }
+  for (int e = i >> 5; e < n; e += kPlanThreads / 32) {
+    const int from = length_of(s, seqs[e]), to = from + counts[e];   // within the held pages: 32 bits
+    const int32_t* row = s.table + static_cast<int64_t>(seqs[e]) * s.max_pages;
+    for (int x = from / s.page_size + (i & 31); x < ceil_div(to, s.page_size) && to > from; x += 32) {
+      const int p = row[x];
+      shared |= p < 0 || p >= s.pages || s.refs[p] != 1;
+    }
+  }
+  if (__syncthreads_or(shared)) {
+    if (i == 0) refuse(s, RB_PAGES_SHARED);
     return;
   }
   if (i < n) s.lengths[seqs[i]] = static_cast<int>(len);

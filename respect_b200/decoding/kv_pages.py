@@ -35,7 +35,7 @@ from respect_b200.kernels.attention import paged_attention
 STATUS = {1: "a sequence that does not exist, is named twice, or is a fork's target in use",
           2: "not enough free pages",
           3: "a count, length, path or position outside the sequence's room",
-          4: "a write into a page that another sequence holds (reserve again after a fork)"}
+          4: "a write or commit into a page that is missing or that another sequence holds (reserve again after a fork)"}
 
 
 class PagedCacheError(RuntimeError):
@@ -152,7 +152,8 @@ class PagedKVCache:
         self._call("rb_kv_pages_write", ctypes.byref(x), s.data_ptr(), None if offsets is None else offsets.data_ptr(), n)
 
     def commit(self, seqs, counts) -> None:
-        """The next counts[i] written tokens of seqs[i] belong to it."""
+        """The next counts[i] written tokens of seqs[i] belong to it. Refused where a write would be:
+        past the reserved room, or on a page that another sequence holds (commit before a fork)."""
         s = self._list(seqs, "seqs")
         c = self._list(counts, "counts", s.numel())
         self._call("rb_kv_pages_commit", s.data_ptr(), c.data_ptr(), s.numel())

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.serving_reference import close
-from tests.test_gpu_serving import BF, F32, i32, paged_inputs, paged_reference
+from tests.test_gpu_serving import BF, DEV, F32, i32, paged_inputs, paged_reference, token_kv
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -62,3 +62,66 @@ def test_a_nan_beside_a_dominating_key_stays(dtype, n, bad, best):
     close(y[max(best, bad):], ref[max(best, bad):], tol.expand(n, -1, -1)[max(best, bad):])
     if best < bad:
         close(y[best:bad], ref[best:bad], tol.expand(n, -1, -1)[best:bad])
+
+
+# ---------------------------------------------------------------- a round that cannot be served
+def test_commit_takes_no_page_that_another_sequence_holds():
+    """A fork, a pool without a free page, and a round of reserve, write and commit without a look at the
+    status in between: nothing grows. After room is made the same round goes through."""
+    from respect_b200.decoding.kv_pages import PagedCacheError, PagedKVCache
+    cache = PagedKVCache(1, 2, 5, 16, 4, dtype=F32)
+    cache.reserve([0, 3], [37, 32])
+    cache.write(*token_kv(cache, list(range(69))), [0, 3], [0, 37, 69])
+    cache.commit([0, 3], [37, 32])
+    cache.fork([0], [1])
+    cache.check()
+    before = [t.clone() for t in (cache.store, cache.table, cache.lengths, cache.held, cache.refs)]
+    seqs, ones = i32([1, 0]), i32([1, 1])
+    new = token_kv(cache, [101, 100])
+    cache.reserve(seqs, ones)
+    cache.write(*new, seqs)
+    cache.commit(seqs, ones)
+    with pytest.raises(PagedCacheError, match="free pages"):
+        cache.check()
+    for a, b in zip(before, (cache.store, cache.table, cache.lengths, cache.held, cache.refs)):
+        assert torch.equal(a, b)
+    cache.commit([0], [1])                                  # alone, too
+    with pytest.raises(PagedCacheError, match="another sequence holds"):
+        cache.check()
+    cache.commit([0, 1], [0, 0])                            # nothing asked: nothing refused
+    cache.check()
+    cache.free([3])
+    cache.reserve(seqs, ones)
+    cache.write(*new, seqs)
+    cache.commit(seqs, ones)
+    cache.check()
+    assert cache.lengths.tolist() == [38, 38, 0, 0]
+    for s, t in ((0, 100), (1, 101)):
+        k, v = token_kv(cache, list(range(37)) + [t])
+        page = cache.table[s].long()[torch.arange(38, device=DEV) // 16]
+        assert torch.equal(cache.store[0, 0, page, :, torch.arange(38, device=DEV) % 16], k[0])
+        assert torch.equal(cache.store[0, 1, page, :, torch.arange(38, device=DEV) % 16], v[0])
+
+
+def test_commit_needs_its_pages():
+    """A page missing from the table refuses the commit; a long commit looks at every page it covers."""
+    from respect_b200.decoding.kv_pages import PagedCacheError, PagedKVCache
+    cache = PagedKVCache(1, 1, 300, 2, 3, dtype=F32, head_dim=8)
+    cache.reserve([0, 1], [400, 20])
+    for at in (0, 77, 199):
+        page = cache.table[0, at].item()
+        cache.table[0, at] = -1
+        cache.commit([1, 0], [20, 400])
+        with pytest.raises(PagedCacheError, match="another sequence holds"):
+            cache.check()
+        cache.table[0, at] = page
+        cache.refs[page] = 2
+        cache.commit([0], [400])
+        with pytest.raises(PagedCacheError, match="another sequence holds"):
+            cache.check()
+        cache.refs[page] = 1
+    assert cache.lengths.tolist() == [0, 0, 0]
+    cache.table[0, 199] = -1
+    cache.commit([1, 0], [20, 398])                         # up to the missing page
+    cache.check()
+    assert cache.lengths.tolist() == [398, 20, 0]
