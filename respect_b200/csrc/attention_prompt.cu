@@ -207,11 +207,13 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
   };
   fetch(0);
   const float* qg = static_cast<const float*>(p.q) + static_cast<int64_t>(s0 + tok0) * p.sqt + kvh * G * p.sqh;
+  // a negative scale's sign goes into Q, so that the largest score has the largest weight
+  const float scale2 = fabsf(p.scale2), sign = p.scale2 < 0.f ? -1.f : 1.f;
   for (int x = threadIdx.x; x < kRows * 32; x += kThreads) {
     const int r = x >> 5, piece = (x & 31) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < rows) v = *reinterpret_cast<const float4*>(qg + r / G * p.sqt + r % G * p.sqh + piece);
-    *reinterpret_cast<float4*>(Q + r * kPitch + piece) = v;
+    *reinterpret_cast<float4*>(Q + r * kPitch + piece) = make_float4(v.x * sign, v.y * sign, v.z * sign, v.w * sign);
   }
   float o[kD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       mx = fmaxf(mx, m[h]);
       const float ref = mx == -INFINITY ? 0.f : mx;
-      alpha[h] = fast_exp2((m[h] - ref) * p.scale2);
+      alpha[h] = fast_exp2((m[h] - ref) * scale2);
       m[h] = mx;
       float sum = 0.f;
 #pragma unroll
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float& x = sc[j][h * 2 + e];
-          x = fast_exp2((x - ref) * p.scale2);   // the difference first: large scores cost no accuracy
+          x = fast_exp2((x - ref) * scale2);   // the difference first: large scores cost no accuracy
           sum += x;
         }
       l[h] = fmaf(l[h], alpha[h], sum);
@@ -863,8 +865,8 @@ int prompt_launch(const rb_prompt_args* a, cudaStream_t st) {
   Dev p{a->q, a->k, a->v, a->sqt, a->sqh, a->skt, a->skh, a->svt, a->svh, a->cu, a->B, a->T, a->H, a->HK,
         a->out, a->sot, a->soh, a->sm_scale * 1.4426950408889634f, (device_sm_count() + a->HK - 1) / a->HK, a->zero_rest};
   const int G = a->H / a->HK;
+  if (a->sm_scale == 0.f) p.scale2 = 1e-37f;   // equal weights; a factor of zero would turn the mask's infinity into a NaN
   if (a->dtype == RB_BF16) {
-    if (a->sm_scale == 0.f) p.scale2 = 1e-37f;   // equal weights; a factor of zero would turn the mask's infinity into a NaN
     const int TP = tcp::kRows / G;
     const int64_t units = (static_cast<int64_t>(a->T) / (2 * TP) + a->B + 1) * a->HK;   // at most
     if (units > INT32_MAX / 2) return RB_ERR_CAPACITY;

@@ -4,10 +4,25 @@ import pytest
 import torch
 
 from tests.serving_reference import close
-from tests.test_gpu_serving import BF, DEV, F32, i32, paged_inputs, paged_reference, token_kv
+from tests.test_gpu_serving import BF, DEV, F32, SCALE, i32, paged_inputs, paged_reference, prompt_inputs, \
+    prompt_reference, token_kv
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
+
+
+def quickest(f, n=3):
+    """Milliseconds of the fastest of n calls after a warm-up."""
+    f()
+    best = INF
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
 
 
 # ---------------------------------------------------------------- scores of minus infinity
@@ -125,3 +140,15 @@ def test_commit_needs_its_pages():
     cache.commit([1, 0], [20, 398])                         # up to the missing page
     cache.check()
     assert cache.lengths.tolist() == [398, 20, 0]
+
+
+# ---------------------------------------------------------------- scales of zero and below
+def test_prompt_scales_of_zero_and_below_cost_no_more():
+    """fp32: the same kernel at the same speed (and right, in a prompt of several tiles)."""
+    from respect_b200.kernels import prompt_attention
+    q, k, v, cu = prompt_inputs(53, [1500, 333], 4, 1, F32)
+    cu_t = i32(cu)
+    plain = quickest(lambda: prompt_attention(q, k, v, cu_t))
+    for scale in (-SCALE, 0.0, -0.25):
+        close(prompt_attention(q, k, v, cu_t, sm_scale=scale), *prompt_reference(q, k, v, cu, scale))
+        assert quickest(lambda: prompt_attention(q, k, v, cu_t, sm_scale=scale)) < 3 * plain + 0.05
