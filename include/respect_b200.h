@@ -125,7 +125,7 @@ RB_API int rb_fused_attn_hyb_noalloc(const rb_attn_args* a, void* stream);
  * tokens [cu[i], cu[i + 1]) (device int32 [B + 1], ascending) of q [T, H, D] and
  * k, v [T, HK, D]; token t of a sequence attends to its tokens 0..t, head h to kv
  * head h / (H / HK). out [T, H, D] of q's type. Rows of no sequence are written as
- * zeros when zero_rest != 0 and left alone otherwise. fp32 accumulation and
+ * zeros when zero_rest != 0 and left alone otherwise; out overlaps no input. fp32 accumulation and
  * softmax statistics; a row's bits do not depend on the packing. Unit inner
  * strides, other strides and bases in whole 16-byte pieces, D = 128,
  * H / HK <= 64. No reference counterpart: its Prefill runs HF's SDPA

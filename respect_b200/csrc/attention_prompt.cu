@@ -92,14 +92,11 @@ __device__ __forceinline__ void zero_rest(const Dev& p, int threads) {   // the 
 // Row `tok` of query head h again, by one warp and key by key. The tiles multiply V
 // rows after the row's own token by a weight of zero, which is not nothing when such
 // a row holds an infinity or a NaN; a row that came out NaN is settled here.
-template <typename T>
 __device__ __noinline__ void redo_row(const Dev& p, int s0, int tok, int h) {
   const int lane = threadIdx.x & 31, d = lane * 4, kvh = h / (p.H / p.HK);
   auto load = [&](const void* base, int64_t at, float (&x)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x[e] = sizeof(T) == 4 ? static_cast<const float*>(base)[at + d + e]
-                            : bf16_bits_to_f32(static_cast<const uint16_t*>(base)[at + d + e]);
+    for (int e = 0; e < 4; ++e) x[e] = static_cast<const float*>(base)[at + d + e];
   };
   float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   load(p.q, static_cast<int64_t>(s0 + tok) * p.sqt + h * p.sqh, q);
@@ -123,8 +120,7 @@ __device__ __noinline__ void redo_row(const Dev& p, int s0, int tok, int h) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int64_t at = static_cast<int64_t>(s0 + tok) * p.sot + h * p.soh + d + e;
-    if (sizeof(T) == 4) static_cast<float*>(p.out)[at] = o[e] / l;
-    else static_cast<uint16_t*>(p.out)[at] = f32_to_bf16_bits(o[e] / l);
+    static_cast<float*>(p.out)[at] = o[e] / l;
   }
 }
 
@@ -322,7 +318,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
     for (int x = 0; again; ++x, again >>= 4)
       if (again & 0xFu) {   // the four lanes of row x
         const int rr = warp * 16 + h * 8 + x;
-        redo_row<float>(p, s0, tok0 + rr / G, kvh * G + rr % G);
+        redo_row(p, s0, tok0 + rr / G, kvh * G + rr % G);
       }
   }
 }
@@ -339,9 +335,15 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
 //
 // Warps 0-3 / 4-7: softmax of tile A / B, one row a thread (no exchange between
 // threads); warp 8: TMA (Q of the block, a ring of K and V tiles); warp 9: issues the
-// MMAs; warp 10: says which tiles are next. The block is persistent: K / V and Q of its
+// MMAs; warp 10: says which tiles are next; warp 11: cleans V. The block is persistent: K / V and Q of its
 // next work item arrive, and S of it is computed, while the results of the last one are
 // written out.
+//
+// A weight of zero does not silence a masked V row that holds an infinity or a NaN. So warp 11
+// looks at the V rows after the item's first token (every row of the item attends to those up to
+// it) while their softmax runs, and clears what is not finite, and rows past the sequence, before
+// their P V. What rows attend to of it is added to the results at the end (restore_rows): at most
+// 2 TP - 1 keys a row, whatever the length, and nothing where V is finite.
 //
 // Bound: the chain S -> softmax -> P V -> next S of a tile (S and P share tensor memory).
 // A step of 128 keys takes about 3,100 cycles, of which the two tiles' four products need
@@ -360,17 +362,25 @@ constexpr int kKVOff = 2 * kTile;                // after Q_A, Q_B
 constexpr int kStageOff = kKVOff + kRing * kTile;  // results on their way out: 32 rows of 64 dims a softmax warp
 constexpr int kBarOff = kStageOff + 8 * 4096;
 constexpr int kItemOff = kBarOff + 256;          // announced items, 32 bytes each
-constexpr int kSmem = 1024 + kItemOff + 64;
+constexpr int kRefOff = kItemOff + 64;           // references of the rows' weights, for restore_rows
+constexpr int kSmem = 1024 + kRefOff + 2 * kRows * 4;
 static_assert(kSmem <= 232448, "shared memory budget");
-constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last warpgroup: TMA, MMA, the work items, an idle warp
+constexpr int kTileThreads = 128, kThreads = 3 * kTileThreads;   // the last warpgroup: TMA, MMA, the work items, V
 // registers a thread: 168 at launch (3 x 128 of them); the softmax warps take what the others leave
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "register split");
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kItemWarp = 10;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kItemWarp = 10, kCleanWarp = 11;
 constexpr int kParts = 2;                        // P is handed over in parts of 128 / kParts keys
 constexpr int kItems = 2;                        // work items announced ahead
 enum { Q_FULL = 0, Q_EMPTY = 1, KV_FULL = 2, KV_EMPTY = KV_FULL + kRing, S_FULL = KV_EMPTY + kRing, P_FULL = S_FULL + 2,
-       O_FULL = P_FULL + 2 * kParts, ITEM_FULL = O_FULL + 2, ITEM_EMPTY = ITEM_FULL + kItems, NBAR = ITEM_EMPTY + kItems };
+       O_FULL = P_FULL + 2 * kParts, ITEM_FULL = O_FULL + 2, ITEM_EMPTY = ITEM_FULL + kItems, V_ASK = ITEM_EMPTY + kItems,
+       V_CLEAN = V_ASK + 2, NBAR = V_CLEAN + 2 };
+static_assert(kRing == 4, "K in the even buffers, V in the odd ones: V_ASK and V_CLEAN of buffer b are number b / 2");
+// Items whose V held something not finite: word i % kOddItems is i + 1 where item i is one. A warp
+// still at item i keeps the others from going past item i + kItems.
+constexpr int kOddItems = 4;
+static_assert(kOddItems > kItems, "a word is not written again before it has been read");
+static_assert(NBAR * 8 + 4 + kOddItems * 4 <= kItemOff - kBarOff, "barriers, TMEM address and flags");
 constexpr uint32_t kSCol = 0, kOCol = 256;       // S_t (and P_t) at 128 t, O_t at 256 + 128 t
 constexpr uint32_t kIdescQK = idesc_bf16_f32(128, 128, 0, 0);
 constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, 0, 1);
@@ -413,6 +423,11 @@ __device__ __forceinline__ bool elect_one() {   // true in one lane of a converg
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
+}
+// Bits 15 and 31: the half is an infinity or a NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) { return ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ void max_abs(uint32_t& m, uint4 x) {   // of bf16 pairs; the signs mean nothing
+  for (const uint32_t w : {x.x, x.y, x.z, x.w}) asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -467,6 +482,52 @@ __device__ __forceinline__ void item_of(const Dev& p, int unit, Item* it) {
     it->n[t] = first < it->len ? (last + kKeys - 1) / kKeys : 0;
   }
 }
+// First K / V tile with a key after the item's first token.
+__device__ __forceinline__ int first_masked(const Item& it) { return (it.tok0 + 1) / kKeys; }
+
+// What a softmax warp's rows attend to of the V entries that the clean warp took out (keys after
+// the item's first token): such an entry makes its dim infinite or NaN. refs: the references of
+// the rows' weights.
+__device__ __noinline__ void restore_rows(const Dev& p, int s0, int len, int tok0, int kvh, const float* refs) {
+  const int G = p.H / p.HK, TP = kRows / G, d = (threadIdx.x & 31) * 4;
+  const int first = tok0 + (threadIdx.x / kRows) * TP, r0 = threadIdx.x / 32 % 4 * 32;   // of the tile: first token; of the warp: first row
+  const int rows = min(TP, len - first) * G;
+  auto load = [&](const void* base, int64_t at) {
+    return *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at + d);
+  };
+  auto value = [](uint2 x, int e) {
+    const uint32_t w = e < 2 ? x.x : x.y;
+    return __uint_as_float((e & 1) ? (w & 0xFFFF0000u) : (w << 16));
+  };
+  for (int r = r0; r < min(rows, r0 + 32); ++r) {
+    const int tok = first + r / G, h = kvh * G + r % G;
+    const float ref = refs[r - r0] == -INFINITY ? 0.f : refs[r - r0];
+    const uint2 q = load(p.q, static_cast<int64_t>(s0 + tok) * p.sqt + h * p.sqh);
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t touched = 0;
+#pragma unroll 4
+    for (int key = tok0 + 1; key <= tok; ++key) {
+      const uint2 v = load(p.v, static_cast<int64_t>(s0 + key) * p.svt + kvh * p.svh);
+      const uint32_t lo = not_finite(v.x), hi = not_finite(v.y);
+      if (!__any_sync(0xffffffffu, lo | hi)) continue;
+      const uint2 k = load(p.k, static_cast<int64_t>(s0 + key) * p.skt + kvh * p.skh);
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dot = fmaf(value(q, e), value(k, e), dot);
+      const float w = fast_exp2(fmaf(warp_sum(dot), p.scale2, -ref));
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((e < 2 ? lo : hi) >> ((e & 1) * 16 + 15) & 1) {
+          add[e] += w * value(v, e);
+          touched |= 1u << e;
+        }
+    }
+    uint16_t* out = static_cast<uint16_t*>(p.out) + static_cast<int64_t>(s0 + tok) * p.sot + h * p.soh + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (touched >> e & 1) out[e] = f32_to_bf16_bits(add[e] + bf16_bits_to_f32(out[e]));
+  }
+}
 }  // namespace tcp
 
 // kFlip: a negative scale, with which the largest weight is at the smallest S.
@@ -479,6 +540,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(psm) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NBAR);
+  volatile int* odd_items = reinterpret_cast<int*>(tmem_slot + 1);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = p.H / p.HK, TP = kRows / G;
@@ -500,7 +562,12 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(bar(ITEM_FULL + i), 1);
-      mbar_init(bar(ITEM_EMPTY + i), 10);   // eight softmax warps, TMA, MMA
+      mbar_init(bar(ITEM_EMPTY + i), 11);   // eight softmax warps, TMA, MMA, V
+    }
+    for (int i = 0; i < kOddItems; ++i) odd_items[i] = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(V_ASK + i), 1);
+      mbar_init(bar(V_CLEAN + i), 1);
     }
     fence_mbar_init();
   }
@@ -516,6 +583,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   pdl_trigger();
   const uint32_t sQ = smem_u32(smem), sKV = smem_u32(smem + kKVOff);
   Item* items = reinterpret_cast<Item*>(smem + kItemOff);
+  float* refs = reinterpret_cast<float*>(smem + kRefOff);
   Item it;
   // The i-th item, as announced; false after the last one (or after a wait gave up).
   auto next_item = [&](int i) {
@@ -553,6 +621,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             const CUtensorMap* m = (x & 1) ? &tv : &tk;
             for (int h = 0; h < 2; ++h)
               tma_load_3d_plain(sKV + b * kTile + h * kHalf, m, bar(KV_FULL + b), h * 64, it.s0 + (x >> 1) * kKeys, it.kvh);
+            if ((x & 1) && (x >> 1) >= first_masked(it)) mbar_arrive(bar(V_ASK + b / 2));
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -570,6 +639,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       const uint64_t dq = sdesc_kmajor_sw128(sQ), dk = sdesc_kmajor_sw128(sKV), dv = sdesc_mnmajor_sw128(sKV, kHalf);
       uint32_t buf = 0, phase = 0;        // of the next K / V tile
       uint32_t steps[2] = {0, 0};         // P tiles of A and B consumed so far
+      uint32_t clean = 0;                 // bit x: parity of V_CLEAN x
       auto advance = [&] {
         if (++buf == kRing) {
           buf = 0;
@@ -601,7 +671,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       };
       bool ok = true;
       for (int i = 0; ok && next_item(i); ++i) {
-        const int n = max(it.n[0], it.n[1]);
+        const int n = max(it.n[0], it.n[1]), masked = first_masked(it);
         ok = mbar_wait_spin(bar(Q_FULL), i & 1, 0x314) && mbar_wait_spin(bar(KV_FULL + buf), phase, 0x313);
         if (!ok) break;
         tc_fence_after();
@@ -618,7 +688,14 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || j >= it.n[t]) continue;
-            if (!v_in) ok = v_in = mbar_wait_spin(bar(KV_FULL + vbuf), vphase, 0x313);
+            if (!v_in) {
+              ok = v_in = mbar_wait_spin(bar(KV_FULL + vbuf), vphase, 0x313);
+              if (ok && j >= masked) {
+                const uint32_t x = vbuf >> 1;
+                ok = mbar_wait_spin(bar(V_CLEAN + x), clean >> x & 1u, 0x318);
+                clean ^= 1u << x;
+              }
+            }
 #pragma unroll
             for (int x = 0; x < kParts; ++x) {
               ok = ok && mbar_wait_spin(bar(P_FULL + t * kParts + x), steps[t] & 1, 0x315);
@@ -658,6 +735,52 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         }
         if (it.n[0] == 0) break;
       }
+    } else {
+      // Of a V tile it is to clean it hears from the TMA warp (V_ASK): a wait on KV_FULL before the
+      // tile's load has begun could take an earlier load's phase for it.
+      uint32_t ring = 0;                  // of the item's K_0
+      uint32_t asked = 0;                 // bit x: parity of V_ASK x
+      bool ok = true;
+      for (int i = 0; ok && next_item(i); ++i) {
+        const int n = max(it.n[0], it.n[1]);
+        bool odd = false;
+        for (int j = first_masked(it); j < n; ++j) {
+          const uint32_t at = ring + 2 * j + 1, b = at % kRing, y = b / 2;
+          ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(V_ASK + y), asked >> y & 1u, 0x31e) &&
+                                           mbar_wait_spin(bar(KV_FULL + b), (at / kRing) & 1, 0x31f));
+          if (!ok) break;
+          asked ^= 1u << y;
+          // half a row a quarter-warp: 16-byte pieces, whose order within a row does not matter
+          uint8_t* v = smem + kKVOff + b * kTile + (lane >> 3 & 1) * kHalf + (lane & 7) * 16;
+          const int from = max(it.tok0 + 1 - j * kKeys, 0) + (lane >> 4), end = min(it.len - j * kKeys, kKeys);
+          uint32_t top = 0;               // largest magnitudes (a NaN if there is one)
+          int r = from;
+          for (; r + 14 < end; r += 16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) max_abs(top, *reinterpret_cast<const uint4*>(v + (r + 2 * e) * 128));
+          }
+          for (; r < end; r += 2) max_abs(top, *reinterpret_cast<const uint4*>(v + r * 128));
+#pragma unroll 4
+          for (r = end + (lane >> 4); r < kKeys; r += 2) *reinterpret_cast<uint4*>(v + r * 128) = make_uint4(0, 0, 0, 0);
+          if (not_finite(top)) {
+            odd = true;
+#pragma unroll 1
+            for (r = from; r < end; r += 2) {
+              uint4 x = *reinterpret_cast<const uint4*>(v + r * 128);
+              x.x &= ~((not_finite(x.x) >> 15) * 0xFFFFu);
+              x.y &= ~((not_finite(x.y) >> 15) * 0xFFFFu);
+              x.z &= ~((not_finite(x.z) >> 15) * 0xFFFFu);
+              x.w &= ~((not_finite(x.w) >> 15) * 0xFFFFu);
+              *reinterpret_cast<uint4*>(v + r * 128) = x;
+            }
+          }
+          if (odd) odd_items[i % kOddItems] = i + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(V_CLEAN + y));
+        }
+        ring += 2 * n;
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -668,10 +791,9 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     const float masked = kFlip ? INFINITY : -INFINITY;
     const uint64_t scale_pair = pair(p.scale2, p.scale2);
     uint32_t step = 0;                                 // S tiles consumed so far
-    uint32_t v_ring = 0;                               // ring number of the item's V_0, less one
     bool ok = true;
     for (int i = 0; ok && next_item(i); ++i) {
-      const int n = it.n[t], N = max(it.n[0], it.n[1]);
+      const int n = it.n[t];
       const int tok = it.tok0 + t * TP + r / G;        // keys <= tok are attended
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++step) {
@@ -726,23 +848,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           }
         }
         m = m_new;
-        if ((j + 1) * kKeys > it.len && (t == 0 || j >= it.n[0])) {
-          // V rows past the sequence are another's: zero weights would not silence what they
-          // hold. The first tile to use this V clears them before its P V is issued.
-          const uint32_t ring = v_ring + 2 * j + 1;
-          ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(KV_FULL + ring % kRing), (ring / kRing) & 1, 0x318));
-          if (!ok) break;
-          uint8_t* v = smem + kKVOff + (ring % kRing) * kTile;
-          if (j * kKeys + r >= it.len) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              *reinterpret_cast<uint4*>(v + r * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(v + kHalf + r * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
         // One straight run of code, so that the exponentials (8 cycles each on their pipe) of one
         // group of 16 overlap the sums, conversions and stores of the group before.
         const uint64_t neg_pair = pair(neg, neg);
@@ -784,7 +889,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         l += a + b;
       }
       const int tok_end = min(it.tok0 + (t + 1) * TP, it.len);
-      v_ring += 2 * N;
       if (n > 0 && ok) {
         ok = __all_sync(0xffffffffu, mbar_wait_spin(bar(O_FULL + t), (step - 1) & 1, 0x319));
         if (!ok) break;
@@ -794,8 +898,8 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         const bool live = r < TP * G && tok < tok_end;
         const int64_t at = live ? static_cast<int64_t>(it.s0 + tok) * p.sot + (it.kvh * G + r % G) * p.soh : -1;
         const float inv = 1.f / l;
+        refs[warp * 32 + lane] = m;
         uint8_t* stage = smem + kStageOff + warp * 4096;
-        bool nan = false;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -809,7 +913,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
                 const float a = __uint_as_float(o[e * 8 + 2 * x]) * inv, b = __uint_as_float(o[e * 8 + 2 * x + 1]) * inv;
-                nan |= a != a || b != b;
                 w[x] = pack_bf16x2(a, b);
               }
               *reinterpret_cast<uint4*>(stage + lane * 128 + (((c * 4 + e) ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -826,10 +929,8 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
           __syncwarp();
         }
         tc_fence_before();   // O read before the next item's P (and so its P V) is announced
-        for (unsigned again = __ballot_sync(0xffffffffu, nan && live); again; again &= again - 1) {
-          const int rr = q4 * 32 + __ffs(again) - 1;
-          redo_row<uint16_t>(p, it.s0, tok - r / G + rr / G, it.kvh * G + rr % G);
-        }
+        if (__any_sync(0xffffffffu, odd_items[i % kOddItems] == i + 1))
+          restore_rows(p, it.s0, it.len, it.tok0, it.kvh, refs + warp * 32);
       }
     }
     if (p.zero_rest) zero_rest<uint16_t>(p, 2 * kTileThreads);

@@ -129,7 +129,8 @@ def prompt_attention(q, k, v, cu_seqlens, sm_scale=None, out=None):
     q [T, H, 128], k, v [T, HK, 128] (bf16 or fp32; slices of a fused projection are
     read in place), cu_seqlens int32 [B + 1] on the same device: sequence i is tokens
     [cu_seqlens[i], cu_seqlens[i + 1]), ascending. Returns [T, H, 128]. Rows of no
-    sequence are zero in a new result and left as they were in a given ``out``."""
+    sequence are zero in a new result and left as they were in a given ``out``, which
+    must not overlap q, k or v."""
     qs, ks = q.shape, k.shape
     if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[0] != qs[0]:
         raise ValueError(f"prompt_attention: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} do not fit")

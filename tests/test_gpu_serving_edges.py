@@ -3,7 +3,7 @@ round, and at sizes that reach the paths of large launches. Tolerances: tests/se
 import pytest
 import torch
 
-from tests.serving_reference import close
+from tests.serving_reference import attention, close
 from tests.test_gpu_serving import BF, DEV, F32, SCALE, i32, paged_inputs, paged_reference, prompt_inputs, \
     prompt_reference, token_kv
 
@@ -152,3 +152,77 @@ def test_prompt_scales_of_zero_and_below_cost_no_more():
     for scale in (-SCALE, 0.0, -0.25):
         close(prompt_attention(q, k, v, cu_t, sm_scale=scale), *prompt_reference(q, k, v, cu, scale))
         assert quickest(lambda: prompt_attention(q, k, v, cu_t, sm_scale=scale)) < 3 * plain + 0.05
+
+
+# ---------------------------------------------------------------- values that are not finite, in prompts
+def with_bad_entries(ref, cu, groups, bad):
+    """A result with V entries (token, kv head, dim, value) added whose weights are not zero."""
+    ref = ref.clone()
+    for token, head, dim, value in bad:
+        end = min(c for c in cu if c > token)
+        ref[token:end, head * groups:(head + 1) * groups, dim] += value
+    return ref
+
+
+@pytest.mark.parametrize("dtype", [BF])
+@pytest.mark.parametrize("H,HK,lens", [(28, 4, [300, 1, 200, 90]), (16, 16, [700, 129, 1]), (64, 1, [40, 150]), (8, 1, [257, 31])])
+def test_prompt_bad_values_at_every_place(dtype, H, HK, lens):
+    """Infinities and NaN in V, several in a tile, on tiles' edges and in the first and last token: only the
+    rows that attend to one show it, in its dim; the others keep their bits."""
+    from respect_b200.kernels import prompt_attention
+    q, k, v, cu = prompt_inputs(61, lens, H, HK, dtype)
+    clean = prompt_attention(q, k, v, i32(cu))
+    ref, tol = prompt_reference(q, k, v, cu)
+    last = cu[-1] - 1
+    for case in ([(0, 0, 3, INF), (5, HK - 1, 127, NAN), (17, 0, 64, -INF), (18, 0, 64, INF)],
+                 [(last, 0, 0, INF), (last, HK - 1, 63, NAN), (last - 1, 0, 0, -INF), (cu[1], 0, 8, -INF)],
+                 [(t, t % HK, t % 128, (INF, -INF, NAN)[t % 3]) for t in range(last + 1)][::9],
+                 [(t, 0, 40, INF) for t in (30, 31, 32, 33, 34)] + [(last - 3, 0, 40, -INF)]):
+        v2, zero = v.clone(), v.clone()
+        for token, head, dim, value in case:
+            v2[token, head, dim], zero[token, head, dim] = value, 0
+        y = prompt_attention(q, k, v2, i32(cu))
+        want, tol2 = prompt_reference(q, k, zero, cu)
+        close(y, with_bad_entries(want, cu, H // HK, case), tol2)
+        untouched = with_bad_entries(torch.zeros_like(ref), cu, H // HK, [(t, h, d, 1.0) for t, h, d, _ in case]) == 0
+        if dtype == BF:
+            assert torch.equal(y[untouched], clean[untouched])
+        assert torch.equal(prompt_attention(q, k, v2, i32(cu)).isnan(), y.isnan())
+    # scores of -inf: such a key weighs nothing; the first token of a prompt has nothing else
+    k2, q2 = k.clone(), q.clone()
+    q2[..., 0] = q2[..., 0].abs() + 1
+    for token in (cu[1], 20, last):
+        k2[token, :, 0] = -INF
+    # their weights are exactly zero on both sides, so what is left is attention over the other keys,
+    # and its bound (the bound over all keys is infinite: it counts |q| |k|)
+    want, tol2 = torch.full_like(ref, NAN), torch.zeros_like(tol)
+    for a, b in zip(cu, cu[1:]):
+        mask = torch.ones(b - a, b - a, dtype=torch.bool, device=DEV).tril()
+        mask &= (k2[a:b, 0, 0] != -INF)[None]
+        some = mask.any(1)
+        o, t = attention(q2[a:b], k2[a:b], v[a:b], mask, SCALE, 2.0 ** -8 if dtype == BF else 0.0)
+        want[a:b][some], tol2[a:b][some] = o[some], t[some]
+    close(prompt_attention(q2, k2, v, i32(cu)), want, tol2)
+
+
+@pytest.mark.parametrize("dtype,H,n", [(BF, 4, 20000), (BF, 2, 150000)])
+def test_prompt_bad_values_cost_little(dtype, H, n):
+    """A NaN that nearly every row of a long prompt attends to, and infinities further on: right, and about as
+    quick as without (a row settled key by key takes longer than the whole call)."""
+    from respect_b200.kernels import prompt_attention
+    q, k, v, cu = prompt_inputs(62, [n], H, 1, dtype)
+    cu = i32(cu)
+    clean = prompt_attention(q, k, v, cu)
+    plain = quickest(lambda: prompt_attention(q, k, v, cu))
+    v = v.clone()
+    v[3, 0, 5], v[n // 2, 0, 7], v[n - 70, 0, 9] = NAN, INF, -INF
+    y = prompt_attention(q, k, v, cu)
+    assert bool(y[3:, :, 5].isnan().all())
+    assert bool((y[n // 2:, :, 7] == INF).all()) and bool((y[n - 70:, :, 9] == -INF).all())
+    same = torch.ones_like(y, dtype=torch.bool)
+    same[3:, :, 5], same[n // 2:, :, 7], same[n - 70:, :, 9] = False, False, False
+    if dtype == BF:
+        assert torch.equal(y[same], clean[same])
+    else:
+        assert bool(((y - clean).abs()[same] <= 1e-5).all())
+    assert quickest(lambda: prompt_attention(q, k, v, cu)) < 3 * plain + 0.1
