@@ -89,46 +89,13 @@ __device__ __forceinline__ void zero_rest(const Dev& p, int threads) {   // the 
   }
 }
 
-// Row `tok` of query head h again, by one warp and key by key. The tiles multiply V
-// rows after the row's own token by a weight of zero, which is not nothing when such
-// a row holds an infinity or a NaN; a row that came out NaN is settled here.
-__device__ __noinline__ void redo_row(const Dev& p, int s0, int tok, int h) {
-  const int lane = threadIdx.x & 31, d = lane * 4, kvh = h / (p.H / p.HK);
-  auto load = [&](const void* base, int64_t at, float (&x)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = static_cast<const float*>(base)[at + d + e];
-  };
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load(p.q, static_cast<int64_t>(s0 + tok) * p.sqt + h * p.sqh, q);
-  for (int j = 0; j <= tok; ++j) {
-    float k[4], v[4];
-    load(p.k, static_cast<int64_t>(s0 + j) * p.skt + kvh * p.skh, k);
-    load(p.v, static_cast<int64_t>(s0 + j) * p.svt + kvh * p.svh, v);
-    const float s = warp_sum(fmaf(q[0], k[0], fmaf(q[1], k[1], fmaf(q[2], k[2], q[3] * k[3])))) * p.scale2;
-    const float mx = fmaxf(m, s), ref = mx == -INFINITY ? 0.f : mx;
-    const float a = fast_exp2(m - ref), w = fast_exp2(s - ref);
-    m = mx;
-    l = fmaf(l, a, w);
-    bool nan = true;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] = fmaf(o[e], a, w * v[e]);
-      nan &= o[e] != o[e];
-    }
-    if (__all_sync(0xffffffffu, nan || l != l)) break;   // nothing changes any more
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t at = static_cast<int64_t>(s0 + tok) * p.sot + h * p.soh + d + e;
-    static_cast<float*>(p.out)[at] = o[e] / l;
-  }
-}
-
 // ---------------------------------------------------------------- fp32
 // Tensor cores with every operand in two tf32 parts (hi hi + hi lo + lo hi: good to
 // about 2^-22 of a product). Four warps of 16 rows; K / V tiles of 32 keys arrive by
 // cp.async one tile ahead. Each step of eight starts from zero and is added to the
 // running sum in fp32, so that sum rounds to nearest however long it gets.
+//
+// A row that comes out NaN is looked at again at the end (settle_rows).
 //
 // Bound: mma.sync, whose pipe is half busy (as are the issue slots: about eight instructions
 // an MMA, two warps a scheduler). Measured: 2,570 tokens of five prompts, 28 / 4 heads, 504 us
@@ -171,13 +138,105 @@ __device__ __forceinline__ void mma3(float (&d)[4], const uint32_t (&ah)[4], con
 __device__ __forceinline__ void copy16(float* dst, const float* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
+
+// The rows of `bad` (bit r: row r came out NaN) again without tensor cores, by the whole block. The
+// tiles give a NaN that the definition does not where a masked V row, multiplied by zero, is not
+// finite, and where an operand is infinite (in two parts, infinity + NaN) or a score's terms
+// overflow. If there is nothing of the kind among what the block's rows read, their NaNs are real.
+// Else a row is taken by two threads, 64 dims each, in the order of its keys. Measured (8,000 tokens,
+// 4 / 1 heads): 1.38 ms; with a NaN that every row attends to 1.65, with an infinity 4.4. Q: the block's queries (staged, with the scale's sign), KV: room for two tiles.
+__device__ __noinline__ void settle_rows(const Dev& p, const float* Q, float* KV, int s0, int len, int tok0, int toks, int kvh,
+                                         uint64_t bad) {
+  const int G = p.H / p.HK, end = tok0 + toks, lane = threadIdx.x & 31;
+  const float* kg = static_cast<const float*>(p.k) + static_cast<int64_t>(s0) * p.skt + kvh * p.skh;
+  const float* vg = static_cast<const float*>(p.v) + static_cast<int64_t>(s0) * p.svt + kvh * p.svh;
+  auto large = [](float4 x) {      // products of two smaller ones cannot overflow in a sum of 128; not NaN
+    return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))) >= 1.152921504606846976e18f;
+  };
+  auto tops = [](float4 x) {       // infinite, or so as its first part
+    return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))) >= 3.4e38f;
+  };
+  bool look = false;
+  for (int x = threadIdx.x; x < kRows * 32; x += kThreads) look |= large(*reinterpret_cast<const float4*>(Q + (x >> 5) * kPitch + (x & 31) * 4));
+  const int rows = min(static_cast<int64_t>(len), (static_cast<int64_t>(end) + kKeys - 1) / kKeys * kKeys);   // whose V the tiles read
+#pragma unroll 4
+  for (int r = threadIdx.x >> 5; r < rows; r += kWarps) {
+    const float4 v = *reinterpret_cast<const float4*>(vg + r * p.svt + lane * 4);
+    look |= tops(v) || (r > tok0 && (v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w));
+    if (r < end) look |= large(*reinterpret_cast<const float4*>(kg + r * p.skt + lane * 4));
+  }
+  if (!__syncthreads_or(look)) return;
+  const int r = threadIdx.x >> 1, half = threadIdx.x & 1, tok = tok0 + r / G;
+  const bool mine = bad >> r & 1;
+  const float scale2 = fabsf(p.scale2);
+  float4 q[kD / 8], o[kD / 8];     // dims 8 i + 4 half
+#pragma unroll
+  for (int i = 0; i < kD / 8; ++i) {
+    q[i] = *reinterpret_cast<const float4*>(Q + r * kPitch + i * 8 + half * 4);
+    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float m = -INFINITY, l = 0.f;
+  auto fetch = [&](int t) {
+    float* K = KV + (t & 1) * 2 * kTile;
+    for (int x = threadIdx.x; x < kKeys * 32; x += kThreads) {
+      const int key = t * kKeys + (x >> 5), to = (x >> 5) * kPitch + (x & 31) * 4;
+      if (key >= end) break;       // read by nobody
+      copy16(K + to, kg + key * p.skt + (x & 31) * 4, 16u);
+      copy16(K + kTile + to, vg + key * p.svt + (x & 31) * 4, 16u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(0);
+  for (int t = 0; t * kKeys < end; ++t) {
+    __syncthreads();               // the other stage has been read
+    fetch(t + 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    // the same keys in every lane of a warp, up to its last row's
+    const int keys = __any_sync(0xffffffffu, mine) ? min(kKeys, __shfl_sync(0xffffffffu, tok, 31) + 1 - t * kKeys) : 0;
+#pragma unroll 1
+    for (int j = 0; j < keys; ++j) {
+      const float* k = KV + (t & 1) * 2 * kTile + j * kPitch + half * 4;
+      const float* v = k + kTile;
+      float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kD / 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(k + i * 8);
+        d = make_float4(fmaf(q[i].x, x.x, d.x), fmaf(q[i].y, x.y, d.y), fmaf(q[i].z, x.z, d.z), fmaf(q[i].w, x.w, d.w));
+      }
+      float s = (d.x + d.y) + (d.z + d.w);
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      if (!mine || t * kKeys + j > tok) continue;
+      const float mx = fmaxf(m, s), ref = mx == -INFINITY ? 0.f : mx;
+      if (mx != m) {
+        const float a = fast_exp2((m - ref) * scale2);
+        l *= a;
+#pragma unroll
+        for (int i = 0; i < kD / 8; ++i) o[i] = make_float4(o[i].x * a, o[i].y * a, o[i].z * a, o[i].w * a);
+        m = mx;
+      }
+      const float w = fast_exp2((s - ref) * scale2);
+      l += w;
+#pragma unroll
+      for (int i = 0; i < kD / 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(v + i * 8);
+        o[i] = make_float4(fmaf(w, x.x, o[i].x), fmaf(w, x.y, o[i].y), fmaf(w, x.z, o[i].z), fmaf(w, x.w, o[i].w));
+      }
+    }
+  }
+  if (!mine) return;
+  float* out = static_cast<float*>(p.out) + static_cast<int64_t>(s0 + tok) * p.sot + (kvh * G + r % G) * p.soh + half * 4;
+#pragma unroll
+  for (int i = 0; i < kD / 8; ++i) *reinterpret_cast<float4*>(out + i * 8) = make_float4(o[i].x / l, o[i].y / l, o[i].z / l, o[i].w / l);
+}
 }  // namespace f32
 
-__global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
+__global__ void __launch_bounds__(f32::kThreads, 2) prompt_f32(const Dev p) {
   using namespace f32;
   extern __shared__ __align__(16) float fsm[];
   float* Q = fsm;
   float* KV = fsm + kRows * kPitch;   // two stages of K, V
+  __shared__ uint32_t bad[kRows / 32];   // rows that came out NaN
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   pdl_wait();
   pdl_trigger();
@@ -202,6 +261,7 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   fetch(0);
+  if (threadIdx.x < kRows / 32) bad[threadIdx.x] = 0;
   const float* qg = static_cast<const float*>(p.q) + static_cast<int64_t>(s0 + tok0) * p.sqt + kvh * G * p.sqh;
   // a negative scale's sign goes into Q, so that the largest score has the largest weight
   const float scale2 = fabsf(p.scale2), sign = p.scale2 < 0.f ? -1.f : 1.f;
@@ -304,8 +364,8 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
     s += __shfl_xor_sync(0xffffffffu, s, 1);
     s += __shfl_xor_sync(0xffffffffu, s, 2);
     const int r = row0 + h * 8;
-    bool nan = false;
     if (r < rows) {   // every row attends to itself: s >= 1, or NaN
+      bool nan = false;
       float* out = static_cast<float*>(p.out) + static_cast<int64_t>(s0 + tok0 + r / G) * p.sot + (kvh * G + r % G) * p.soh;
 #pragma unroll
       for (int n = 0; n < kD / 8; ++n) {
@@ -313,14 +373,11 @@ __global__ void __launch_bounds__(f32::kThreads) prompt_f32(const Dev p) {
         nan |= y.x != y.x || y.y != y.y;
         *reinterpret_cast<float2*>(out + n * 8 + c * 2) = y;
       }
+      if (nan) atomicOr(&bad[r >> 5], 1u << (r & 31));
     }
-    unsigned again = __ballot_sync(0xffffffffu, nan);
-    for (int x = 0; again; ++x, again >>= 4)
-      if (again & 0xFu) {   // the four lanes of row x
-        const int rr = warp * 16 + h * 8 + x;
-        redo_row(p, s0, tok0 + rr / G, kvh * G + rr % G);
-      }
   }
+  __syncthreads();
+  if (bad[0] | bad[1]) settle_rows(p, Q, KV, s0, len, tok0, toks, kvh, bad[0] | static_cast<uint64_t>(bad[1]) << 32);
 }
 
 // ---------------------------------------------------------------- bf16

@@ -164,7 +164,7 @@ def with_bad_entries(ref, cu, groups, bad):
     return ref
 
 
-@pytest.mark.parametrize("dtype", [BF])
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("H,HK,lens", [(28, 4, [300, 1, 200, 90]), (16, 16, [700, 129, 1]), (64, 1, [40, 150]), (8, 1, [257, 31])])
 def test_prompt_bad_values_at_every_place(dtype, H, HK, lens):
     """Infinities and NaN in V, several in a tile, on tiles' edges and in the first and last token: only the
@@ -205,10 +205,11 @@ def test_prompt_bad_values_at_every_place(dtype, H, HK, lens):
     close(prompt_attention(q2, k2, v, i32(cu)), want, tol2)
 
 
-@pytest.mark.parametrize("dtype,H,n", [(BF, 4, 20000), (BF, 2, 150000)])
+@pytest.mark.parametrize("dtype,H,n", [(BF, 4, 20000), (BF, 2, 150000), (F32, 4, 20000)])
 def test_prompt_bad_values_cost_little(dtype, H, n):
-    """A NaN that nearly every row of a long prompt attends to, and infinities further on: right, and about as
-    quick as without (a row settled key by key takes longer than the whole call)."""
+    """A NaN that nearly every row of a long prompt attends to, and infinities further on: right, and within a
+    small factor of the call without (fp32 goes over infinities a second time; rows settled one by one and key by
+    key took hundreds of times as long)."""
     from respect_b200.kernels import prompt_attention
     q, k, v, cu = prompt_inputs(62, [n], H, 1, dtype)
     cu = i32(cu)
@@ -225,4 +226,4 @@ def test_prompt_bad_values_cost_little(dtype, H, n):
         assert torch.equal(y[same], clean[same])
     else:
         assert bool(((y - clean).abs()[same] <= 1e-5).all())
-    assert quickest(lambda: prompt_attention(q, k, v, cu)) < 3 * plain + 0.1
+    assert quickest(lambda: prompt_attention(q, k, v, cu)) < (3 if dtype == BF else 6) * plain + 0.1
