@@ -544,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 8)
             }
             const unsigned again = __ballot_sync(0xffffffffu, nan);
             if (again) {
+              __syncwarp();   // the row's first result is in place before the second
               for (int x = 0; x < 4; ++x)
                 if (again & (0x11111111u << x)) redo_row<T>(p, it, part, n * 8 + x * 2 + e, chunk);
             }

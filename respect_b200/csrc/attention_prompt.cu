@@ -144,7 +144,8 @@ __device__ __forceinline__ void copy16(float* dst, const float* src, uint32_t by
 // finite, and where an operand is infinite (in two parts, infinity + NaN) or a score's terms
 // overflow. If there is nothing of the kind among what the block's rows read, their NaNs are real.
 // Else a row is taken by two threads, 64 dims each, in the order of its keys. Measured (8,000 tokens,
-// 4 / 1 heads): 1.38 ms; with a NaN that every row attends to 1.65, with an infinity 4.4. Q: the block's queries (staged, with the scale's sign), KV: room for two tiles.
+// 4 / 1 heads): 1.38 ms; with a NaN that every row attends to 1.65, with an infinity 4.4.
+// Q: the block's queries (staged, with the scale's sign), KV: room for two tiles.
 __device__ __noinline__ void settle_rows(const Dev& p, const float* Q, float* KV, int s0, int len, int tok0, int toks, int kvh,
                                          uint64_t bad) {
   const int G = p.H / p.HK, end = tok0 + toks, lane = threadIdx.x & 31;
