@@ -3,9 +3,10 @@ round, and at sizes that reach the paths of large launches. Tolerances: tests/se
 import pytest
 import torch
 
+from tests import test_gpu_serving as base
 from tests.serving_reference import attention, close
-from tests.test_gpu_serving import BF, DEV, F32, SCALE, i32, paged_inputs, paged_reference, prompt_inputs, \
-    prompt_reference, token_kv
+from tests.test_gpu_serving import BF, DEV, F32, SCALE, gen, i32, paged_inputs, paged_reference, prompt_inputs, \
+    prompt_reference, randn, token_kv
 
 pytestmark = pytest.mark.gpu
 NAN, INF = float("nan"), float("inf")
@@ -227,3 +228,200 @@ def test_prompt_bad_values_cost_little(dtype, H, n):
     else:
         assert bool(((y - clean).abs()[same] <= 1e-5).all())
     assert quickest(lambda: prompt_attention(q, k, v, cu)) < (3 if dtype == BF else 6) * plain + 0.1
+
+
+# ---------------------------------------------------------------- sizes of large launches
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("ps", [16, 24])
+def test_paged_warps_that_take_several_chunks(dtype, ps):
+    """Enough chunks in one call that a warp takes several of them: every row has the bits of a call of its
+    own, in which a warp takes one."""
+    from respect_b200.kernels import paged_attention
+    lens = [2500, 1, 700, 2047, 130, 0]
+    q, k, v, table, seqs = paged_inputs(54, lens, 16, 8, ps, dtype)
+    ref, tol = paged_reference(q, seqs)
+    pick = [i % 6 for i in range(96)]                       # 96 x 8 heads x 40 chunks (bf16) or 79 (fp32)
+    y = paged_attention(q[pick], k, v, table, i32(lens), seqs=i32(pick))
+    for row, i in enumerate(pick):
+        if row < 6:
+            close(y[i], ref[i], tol[i])
+            assert torch.equal(paged_attention(q[i:i + 1], k, v, table, i32(lens), seqs=i32([i]))[0], y[i])
+        else:
+            assert torch.equal(y[row], y[i])
+
+
+@pytest.mark.parametrize("H,HK,lens", [(16, 16, [6000, 300, 1, 2900]), (32, 8, [2500, 0, 6100, 33, 700]), (28, 4, [4100, 3000])])
+def test_prompt_blocks_with_several_items_and_bands(H, HK, lens):
+    """More work items than blocks (three and more a block) and prompts longer than a band of tiles."""
+    from respect_b200.kernels import prompt_attention
+    q, k, v, cu = prompt_inputs(55 + H, lens, H, HK, BF)
+    y = prompt_attention(q, k, v, i32(cu))
+    close(y, *prompt_reference(q, k, v, cu))
+    for a, b in zip(cu, cu[1:]):
+        assert torch.equal(prompt_attention(q[a:b], k[a:b], v[a:b], i32([0, b - a])), y[a:b])
+
+
+@pytest.mark.parametrize("tokens,layers", [(700, 8), (801, 28)])
+def test_page_writes_of_several_layers_a_warp(tokens, layers):
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    cache = PagedKVCache(layers, 2, 150, 16, 2, dtype=F32, head_dim=20)
+    cut = tokens // 3
+    cache.reserve([1, 0], [cut, tokens - cut])
+    k, v = token_kv(cache, list(range(tokens)))
+    cache.write(k, v, [1, 0], [0, cut, tokens])
+    cache.commit([1, 0], [cut, tokens - cut])
+    cache.check()
+    for s, a, b in ((1, 0, cut), (0, cut, tokens)):
+        pos = torch.arange(b - a, device=DEV)
+        page, slot = cache.table[s].long()[pos // 16], pos % 16
+        assert torch.equal(cache.store[:, 0][:, page, :, slot].transpose(0, 1), k[:, a:b])
+        assert torch.equal(cache.store[:, 1][:, page, :, slot].transpose(0, 1), v[:, a:b])
+
+
+def test_reserve_looks_through_a_large_pool():
+    """More pages than one look of the planning block: the lowest free ones, in list order."""
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    pages = 9001
+    cache = PagedKVCache(1, 1, pages, 1, 4, dtype=F32, head_dim=4)
+    free = torch.rand(pages, device=DEV, generator=gen(56)) < 0.6
+    cache.refs.copy_(torch.where(free, 0, 1))
+    low = free.nonzero()[:, 0].tolist()
+    counts = [1, 2500, 0, 2600]
+    cache.reserve([2, 0, 1, 3], counts)
+    cache.check()
+    at = 0
+    for s, n in zip([2, 0, 1, 3], counts):
+        assert cache.table[s, :n].tolist() == low[at:at + n] and bool((cache.table[s, n:] == -1).all())
+        at += n
+    assert cache.refs.nonzero()[:, 0].tolist() == sorted(low[:at] + (~free).nonzero()[:, 0].tolist())
+
+
+def test_compact_of_long_paths():
+    """Paths longer than the tokens a block looks up at a time."""
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    cache = PagedKVCache(2, 2, 100, 16, 2, dtype=F32)
+    cache.reserve([0, 1], [9, 500])
+    cache.write(*token_kv(cache, list(range(509))), [0, 1], [0, 9, 509])
+    path = sorted(torch.randperm(500, generator=torch.Generator().manual_seed(57))[:300].tolist())
+    cache.compact([1, 0], [path, [0, 4, 8]], [300, 3])
+    cache.check()
+    assert cache.lengths.tolist() == [3, 300]
+    for s, tokens in ((1, [9 + t for t in path]), (0, [0, 4, 8])):
+        pos = torch.arange(len(tokens), device=DEV)
+        page, slot = cache.table[s].long()[pos // 16], pos % 16
+        k, v = token_kv(cache, tokens)
+        assert torch.equal(cache.store[:, 0][:, page, :, slot].transpose(0, 1), k)
+        assert torch.equal(cache.store[:, 1][:, page, :, slot].transpose(0, 1), v)
+
+
+@pytest.mark.parametrize("ps,pages,layers,heads,dim", [(16, 30, 2, 3, 128), (5, 70, 3, 1, 8)])
+def test_page_operations_follow_the_model_in_bf16(monkeypatch, ps, pages, layers, heads, dim):
+    """The model test with values that bf16 holds exactly: a token's number in digits of base 16."""
+    def digits(cache, tokens):
+        t = torch.tensor(tokens, device=DEV, dtype=torch.int64).reshape(1, -1, 1, 1)
+        part = torch.arange(cache.layers * cache.kv_heads, device=DEV).reshape(cache.layers, 1, cache.kv_heads, 1)
+        d = torch.arange(cache.head_dim, device=DEV)
+        k = ((t >> (d % 4 * 4) & 15) + 16 * (part % 16)).to(cache.dtype)
+        return k, -k - 1
+    monkeypatch.setattr(base, "token_kv", digits)
+    base.test_page_operations_follow_the_model(ps, pages, BF, layers, heads, dim)
+
+
+def test_page_operations_past_32_bits():
+    """Pages whose elements lie beyond 2^31: written, copied for a fork, compacted and given back."""
+    from respect_b200.decoding.kv_pages import PagedKVCache
+    pages, low = 70000, 69980
+    store = torch.empty(1, 2, pages, 4, 64, 128, device=DEV, dtype=BF)      # 4.6e9 elements
+    z = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)
+    refs = z(pages)
+    refs[:low] = 1
+    cache = PagedKVCache.from_state(store, z(3, 8) - 1, z(3), z(3), refs)
+    k, v = randn(gen(58), 2, 1, 300, 4, 128, dtype=BF)
+    cache.reserve([2], [100])
+    cache.write(k[:, :100], v[:, :100], [2], [0, 100])
+    cache.commit([2], [100])
+    cache.fork([2], [0])
+    cache.reserve([0], [200])                                  # copies the last page
+    cache.write(k[:, 100:], v[:, 100:], [0], [0, 200])
+    path = list(range(1, 200, 3))
+    cache.compact([0], [path], [len(path)])
+    cache.check()
+    assert cache.table[2, :2].tolist() == [low, low + 1] and cache.table[0, :2].tolist() == [low, low + 2]
+    for s, tokens in ((2, list(range(100))), (0, list(range(100)) + [100 + t for t in path])):
+        pos = torch.arange(len(tokens), device=DEV)
+        page, slot = cache.table[s].long()[pos // 64], pos % 64
+        assert torch.equal(store[0, 0][page, :, slot], k[0, tokens]) and torch.equal(store[0, 1][page, :, slot], v[0, tokens])
+    cache.free([0, 2])
+    assert bool((refs[:low] == 1).all()) and not bool(refs[low:].any())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_prompts(dtype):
+    """Thousands of prompts of a few tokens, many of them empty."""
+    from respect_b200.kernels import prompt_attention
+    lens = torch.randint(0, 6, (3000,), generator=torch.Generator().manual_seed(59)).tolist()
+    lens[1700] = 200
+    q, k, v, cu = prompt_inputs(59, lens, 8, 2, dtype, before=3, behind=2)
+    y = prompt_attention(q, k, v, i32(cu))
+    T = q.shape[0]
+    owner = torch.bucketize(torch.arange(T, device=DEV), i32(cu), right=True)      # 0: before, 3001: behind
+    mask = (owner[:, None] == owner[None]) & torch.ones(T, T, dtype=torch.bool, device=DEV).tril()
+    mask[owner == 0], mask[owner == 3001] = False, False
+    for r in range(0, T, 1024):
+        close(y[r:r + 1024], *attention(q[r:r + 1024], k, v, mask[r:r + 1024], SCALE, 2.0 ** -8 if dtype == BF else 0.0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_paged_wide_groups_and_pages(dtype):
+    """Groups past a block's sixteen heads, pages longer than most sequences, many sequences of one row each."""
+    from respect_b200.kernels import paged_attention
+    for H, HK, ps, lens in ((70, 2, 1000, [1700, 3, 999, 1001]), (17, 1, 48, [49, 0, 400])):
+        q, k, v, table, seqs = paged_inputs(60 + H, lens, H, HK, ps, dtype)
+        close(paged_attention(q, k, v, table, i32(lens)), *paged_reference(q, seqs))
+    lens = [i % 40 for i in range(700)]
+    q, k, v, table, seqs = paged_inputs(63, lens, 4, 1, 16, dtype)
+    y = paged_attention(q, k, v, table, i32(lens))
+    for b in (0, 1, 39, 355, 699):
+        o, t = paged_reference(q[b:b + 1], seqs[b:b + 1])
+        close(y[b:b + 1], o, t)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_token_logprobs_many_rows_and_past_32_bits(dtype):
+    """More rows than a grid's second dimension could hold, and logits whose elements lie beyond 2^31: the
+    bits of the same rows alone."""
+    from respect_b200.decoding.acceptance import token_logprobs
+    g = gen(64)
+    for rows, V, top in ((70000, 50, 3), (15000, 152064, 5)):
+        x = torch.empty(rows, V, device=DEV, dtype=dtype)
+        for r in range(0, rows, 4096):
+            x[r:r + 4096] = randn(g, *x[r:r + 4096].shape, dtype=dtype, scale=3.0)
+        tokens = torch.randint(0, V, (rows,), device=DEV, generator=g)
+        r = token_logprobs(x, tokens, top, 7, 20)
+        some = [0, 1, rows // 2, rows - 2, rows - 1]
+        one = token_logprobs(x[some], tokens[some], top, 7, 20)
+        tokens_out = (tokens[some] >= 7) & (tokens[some] < 27)      # -inf: equal, too
+        assert all(torch.equal(a[some], b) for a, b in zip(r, one)) and bool((r.logprob[some].isinf() == tokens_out).all())
+        base.assert_logprobs(x[some], tokens[some], top, 7, 20)
+        del x, r
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_token_logprobs_masked_by_the_lowest_value(dtype):
+    """Entries at the type's lowest value weigh what entries at -inf weigh; a row of nothing else is uniform."""
+    from respect_b200.decoding.acceptance import token_logprobs
+    V = 30001
+    g = gen(65)
+    x = randn(g, 4, V, dtype=dtype, scale=3.0)
+    tokens = torch.tensor([5, 20000, 17, 3], device=DEV)
+    masked = torch.rand(4, V, device=DEV, generator=g) < 0.7
+    masked[1, 8192:16384] = True
+    masked[torch.arange(4), tokens] = False
+    low = x.masked_fill(masked, torch.finfo(dtype).min)
+    a, b = token_logprobs(low, tokens, 20), token_logprobs(x.masked_fill(masked, -INF), tokens, 20)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+    r = token_logprobs(torch.full_like(x, torch.finfo(dtype).min), tokens, 4)
+    want = torch.full((4,), float(V), device=DEV).log()
+    # log S of V ones: S good to 2^-17 (see assert_logprobs), and the logarithm's own rounding
+    assert bool(((r.logprob + want).abs() <= 2.0 ** -17).all()) and bool(((r.entropy - want).abs() <= 2.0 ** -17).all())
+    assert r.top_ids.tolist() == [[0, 1, 2, 3]] * 4
