@@ -18,7 +18,7 @@
 //
 // Measured (both launches, one B200): 64 bf16 sequences of 512 to 12,000 tokens, 32 / 8 heads,
 // 286 us = 5.5 TB/s (with heads as rows and blocks of four warps 335); 256 of 1,024 tokens 5.1
-// TB/s; one of 120,000 4.9 TB/s; one of 4,133, 28 / 4 heads, 14 us, of which most is latency.
+// TB/s; one of 120,000 4.7 TB/s; one of 4,133, 28 / 4 heads, 14 us, of which most is latency.
 #include <type_traits>
 
 #include "common.cuh"
@@ -36,7 +36,8 @@ constexpr int kMinChunk = 32, kMaxChunk = 2048;
 // Keys per chunk of a sequence of `len` tokens: in bf16 64 up to 4,096 tokens, then doubled
 // each time the length is four times larger; in fp32, whose keys are twice as long and cost
 // several times the instructions, 32 up to 16,384. A chunk's result costs G x 520 bytes written and read against 512 bytes a key
-// (bf16): 6% of the traffic for a group of 4 at 64.
+// (bf16): 6% of the traffic for a group of 4 at 64. A single sequence pays where the size doubles, as half
+// as many warps read it: 4,096 tokens of 28 / 4 heads take 11.6 us, 4,097 take 14.6.
 __host__ __device__ constexpr int kGrow(int es) { return es == 2 ? 1 : 16; }
 __host__ __device__ inline int chunk_of(int len, int es) {
   int c = kMinChunk * 4 / es;

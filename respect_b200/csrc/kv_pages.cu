@@ -8,7 +8,8 @@
 // plans a call and as few launches as the order of the steps allows, chained by
 // programmatic dependent launch. A call is all or nothing: the plan checks every
 // entry first, and a call that cannot be served raises the state's status word and
-// changes nothing.
+// changes nothing. Writing has no plan: it leaves out the tokens that have no place, and
+// a commit of such a token is refused.
 //
 // Measured (28 layers, 4 kv heads of 128, bf16, pages of 16): 1,024 drafted tokens of four
 // sequences truncated, reserved, written (59 MB in, 59 MB out) and compacted 36 us; 16

@@ -20,8 +20,9 @@ A round of decoding:
 Operations take sequence numbers and counts as int32 tensors on the cache's device
 (lists are copied there). A call that cannot be served (no free page, a sequence
 named twice, a count outside the room) changes nothing and raises the cache's status
-word; ``check()`` reads it and raises. Calls on one cache must be ordered: one
-stream, or events between streams.
+word; ``check()`` reads it and raises. Only ``write`` works token by token: it leaves out
+those that have no place of their own, and ``commit`` refuses them. Calls on one cache must
+be ordered: one stream, or events between streams.
 """
 from __future__ import annotations
 
@@ -124,7 +125,8 @@ class PagedKVCache:
         self._call("rb_kv_pages_reserve", s.data_ptr(), c.data_ptr(), s.numel(), self._ws.data_ptr(), self._ws_bytes)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, seqs, offsets=None, layer: int | None = None) -> None:
-        """K and V of new tokens to the positions after the committed ones, inside reserved room:
+        """K and V of new tokens to the positions after the committed ones, inside reserved room
+        (tokens outside it, or on a page that another sequence holds, are left out and raise the status):
         tokens [offsets[i], offsets[i + 1]) belong to seqs[i] (default: one token each). k, v
         [tokens, kv_heads, head_dim] for one ``layer``, [layers, tokens, kv_heads, head_dim] for all."""
         s = self._list(seqs, "seqs")
@@ -201,7 +203,10 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, seqs, layer: int, ahead: int = 0, sm_scale: float | None = None,
                max_length: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """paged_attention of q [n, H, head_dim] over the tokens of seqs in one layer: the
-        committed ones and ``ahead`` written after them."""
+        committed ones and ``ahead`` written after them. Without a ``max_length`` scratch and launch
+        are sized for max_pages * page_size tokens a sequence: 64 sequences of 512 tokens, 28 / 4
+        heads, in a cache of 4,096 pages of 16 take 67 us and 239 MB of scratch, with max_length=1024
+        32 us and 15 MB."""
         k, v = self.layer_kv(layer)
         return paged_attention(q, k, v, self.table, self.lengths, sm_scale, self._list(seqs, "seqs"), ahead, max_length,
                                out)
