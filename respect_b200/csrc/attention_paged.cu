@@ -635,7 +635,7 @@ static int paged_validate(const rb_paged_args* a) {
   if ((a->dtype != RB_BF16 && a->dtype != RB_F32) || a->D != pg::kD || a->H % a->HK != 0) return RB_ERR_UNSUPPORTED;
   if (a->B > 65535 || a->H > 65535 || static_cast<int64_t>(a->width) * a->page_size > (INT64_C(1) << 30)) return RB_ERR_CAPACITY;
   if (a->B == 0) return RB_OK;
-  if (!a->q || !a->out || !a->lengths || (a->width > 0 && !a->table) || (a->pages > 0 && (!a->k || !a->v)))
+  if (!a->q || !a->out || (a->rows > 0 && (!a->lengths || (a->width > 0 && !a->table))) || (a->pages > 0 && (!a->k || !a->v)))
     return RB_ERR_INVALID_ARG;
   const int es = a->dtype == RB_BF16 ? 2 : 4;
   for (int64_t s : {a->sqb, a->sqh, a->skp, a->skh, a->sks, a->svp, a->svh, a->svs, a->sob, a->soh})

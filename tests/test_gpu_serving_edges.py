@@ -425,3 +425,51 @@ def test_token_logprobs_masked_by_the_lowest_value(dtype):
     # log S of V ones: S good to 2^-17 (see assert_logprobs), and the logarithm's own rounding
     assert bool(((r.logprob + want).abs() <= 2.0 ** -17).all()) and bool(((r.entropy - want).abs() <= 2.0 ** -17).all())
     assert r.top_ids.tolist() == [[0, 1, 2, 3]] * 4
+
+
+# ---------------------------------------------------------------- calls that nothing above makes
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_tables_without_columns_or_rows(dtype):
+    from respect_b200.kernels import paged_attention
+    q, k, v, table, _ = paged_inputs(66, [30, 5], 8, 2, 16, dtype)
+    assert not bool(paged_attention(q, k, v, table[:, :0], i32([30, 5])).any())
+    assert not bool(paged_attention(q, k, v, table[:0], i32([]), seqs=i32([0, 1])).any())
+    assert not bool(paged_attention(q, k[:0], v[:0], table, i32([30, 5])).any())
+    assert not bool(paged_attention(q, k, v, table, i32([0, -7]), ahead=0).any())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_two_streams_at_once_and_a_captured_call_with_bad_values(dtype):
+    """The same operators on two streams at a time, and a graph whose replay meets values that are not finite."""
+    from respect_b200.decoding.acceptance import token_logprobs
+    from respect_b200.kernels import paged_attention, prompt_attention
+    q, k, v, cu = prompt_inputs(67, [900, 300], 8, 2, dtype)
+    v, cu = v.clone(), i32(cu)
+    pq, pk, pv, table, _ = paged_inputs(68, [3000, 700], 8, 2, 16, dtype)
+    n = i32([3000, 700])
+    x, tok = randn(gen(69), 40, 30000, dtype=dtype), torch.arange(40, device=DEV)
+
+    def everything():
+        return (prompt_attention(q, k, v, cu), paged_attention(pq, pk, pv, table, n), *token_logprobs(x, tok, 7))
+
+    want = everything()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(everything())
+    torch.cuda.synchronize()
+    for y in got:
+        assert all(torch.equal(a, b) for a, b in zip(y, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = prompt_attention(q, k, v, cu)
+    for token, value in ((890, NAN), (5, INF), (1000, -INF)):
+        v[token, 1, 17] = value
+        graph.replay()
+        again = prompt_attention(q, k, v, cu)
+        assert torch.equal(y.nan_to_num(7.0), again.nan_to_num(7.0)) and torch.equal(y.isnan(), again.isnan())
+        assert not torch.equal(y[token:token + 1], want[0][token:token + 1])
